@@ -82,7 +82,8 @@ const char* vit_last_error(void);
 /* ABI version: bumped when an entry point is added or a signature changes. History: 1 = inference path and
  * per-kernel entry points; 2 = + training step, folded LayerNorm, heads, preprocessing, position interpolation,
  * vit_forward_static; 3 = vit_backward_stage accepts any stash that a vit_forward_train of this context filled
- * (several in flight), few-tile GEMM route. The library returns the VIT_ABI_VERSION it was built with. */
+ * (several in flight), few-tile GEMM route; the head norm / rotation and relative-position-bias entry points joined it
+ * without a change to any earlier signature. The library returns the VIT_ABI_VERSION it was built with. */
 #define VIT_ABI_VERSION 3
 int vit_abi_version(void);
 
@@ -228,6 +229,67 @@ int vit_attention_bwd(const void* qkv, const void* out, const void* d_out, const
  * gradient of the skip branch, MV:277,284); dgamma / dbeta are ACCUMULATED (+=, fp32 atomics). */
 int vit_layernorm_bwd(const void* x, const void* dy, const float* gamma, const void* d_residual, void* dx,
                       float* dgamma, float* dbeta, int rows, int dim, float eps, void* stream);
+
+/* ---- the step between the QKV projection and attention: norm of every query and key head and the rotary rotation of
+ * its position, one pass over the packed rows [batch * seq, (heads + 2 kv_heads) * head_dim] (q heads | k heads | v heads):
+ *   xh = (x - mean) / sqrt(var + eps)  (VIT_NORM_LAYER; biased variance)  or  x / sqrt(mean(x^2) + eps)  (VIT_NORM_RMS)
+ *   out = R(position) (xh * weight + bias), the first rot_dim values of a head turned in pairs: (i, i + rot_dim / 2), or
+ *   neighbours (2 i, 2 i + 1) with `interleaved`;  (a, b) -> (a cos - b sin, b cos + a sin).
+ * Value heads pass through. weights / biases are fp32 [head_dim], shared by all heads (biases: LAYER only, may be NULL).
+ * `rope` is fp32 [rope_len, rot_dim / 2, 2] = (cos, sin); a token's row is positions[token] (int32 [seq], or [batch, seq]
+ * with positions_per_sample), its place in the sequence when positions is NULL. A position outside [0, rope_len) leaves the
+ * token unturned (CLS and register tokens: -1). head_dim % 16 == 0, <= 128; rot_dim % 16 == 0, 0 = no rotation. */
+#define VIT_NORM_RMS 0
+#define VIT_NORM_LAYER 1
+typedef struct vit_qk_norm_config {
+    int32_t batch, seq, heads, kv_heads, head_dim;
+    int32_t norm;                 /* VIT_NORM_* */
+    int32_t rot_dim, interleaved;
+    int32_t rope_len;             /* rows of `rope` */
+    int32_t positions_per_sample; /* positions: 0 = [seq], 1 = [batch, seq] */
+    int32_t dtype;                /* VIT_F32 | VIT_BF16: qkv, out and their gradients */
+    float eps;                    /* > 0 */
+} vit_qk_norm_config;
+/* `out` may be `qkv` itself (the values are then not touched); any other overlap is refused. */
+int vit_qk_norm_rope_fwd(const vit_qk_norm_config* cfg, const void* qkv, const float* q_weight, const float* k_weight,
+                         const float* q_bias, const float* k_bias, const float* rope, const int32_t* positions, void* out,
+                         void* stream);
+/* Gradients from the UN-normalised qkv and the gradient d_out of the packed output: dqkv (may be d_out itself; its value part
+ * is d_out's) and the parameters' fp32 sums over all tokens and heads, overwritten (bias ones may be NULL). No atomics. */
+size_t vit_qk_norm_rope_bwd_workspace_bytes(const vit_qk_norm_config* cfg);
+int vit_qk_norm_rope_bwd(const vit_qk_norm_config* cfg, const void* qkv, const void* d_out, const float* q_weight,
+                         const float* k_weight, const float* rope, const int32_t* positions, void* dqkv, float* dq_weight,
+                         float* dk_weight, float* dq_bias, float* dk_bias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- attention with a learned relative position bias by buckets:
+ *   out = softmax(scale Q K^T + bias) V,   bias[i, j] of head h = table[bucket(i, j) * heads + h]
+ * The tokens are `prefix` tokens without a place (CLS, registers), then a grid_h x grid_w grid in row order (a sequence is
+ * 1 x n). Two grid tokens, row / column offset (dy, dx) = place of query - place of key, have the offset index
+ *   (dy + grid_h - 1) (2 grid_w - 1) + dx + grid_w - 1;
+ * three more indices follow the (2 grid_h - 1)(2 grid_w - 1) offsets: prefix query on a grid key, grid query on a prefix key,
+ * prefix on prefix. bucket = bucket_of[index], or the index itself when bucket_of is NULL (a bucket outside [0, num_buckets)
+ * biases nothing). A table entry below -1e30 masks its pairs; a query left without a key gives zeros. */
+typedef struct vit_rel_pos {
+    int32_t prefix, grid_h, grid_w; /* 0 <= prefix <= 32; seq = prefix + grid_h * grid_w */
+    int32_t num_buckets;
+    const int32_t* bucket_of;    /* device [offsets (+ 3 with a prefix)] or NULL */
+    const int32_t* by_bucket;    /* device: the indices sorted by bucket, and where each bucket starts in them */
+    const int32_t* bucket_start; /* [num_buckets + 1]; both only for d_table with bucket_of */
+} vit_rel_pos;
+/* qkv: packed as above (query head h reads key / value head h / (heads / kv_heads)); out [batch * seq, heads * head_dim];
+ * lengths: int32 [batch] device, tokens in use of each sample (keys behind are not read, rows behind give zeros), or NULL.
+ * lse (VIT_BF16 only, may be NULL): [batch, heads, seq], the base-2 log-sum-exp that the backward takes (+inf where there
+ * is no key). A grid too large for the LDS expansion of a query block's offsets (16384 entries:
+ * beyond 88 x 88, or 1 x 16128 tokens) is refused. */
+int vit_attention_rel_fwd(const vit_rel_pos* pos, const void* qkv, const float* table, const int32_t* lengths, void* out,
+                          float* lse, int batch, int heads, int kv_heads, int head_dim, float scale, int dtype,
+                          void* stream);
+/* VIT_BF16. dqkv (rows behind a sample's length: zeros) and d_table [num_buckets, heads] fp32, overwritten; d_table may be
+ * NULL. No atomics: bitwise reproducible. */
+size_t vit_attention_rel_bwd_workspace_bytes(const vit_rel_pos* pos, int batch, int heads);
+int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, const float* table, const int32_t* lengths, const void* out,
+                          const void* d_out, const float* lse, void* dqkv, float* d_table, void* workspace,
+                          size_t workspace_bytes, int batch, int heads, int kv_heads, int head_dim, float scale, void* stream);
 
 /* dst[C, Rpad] = src[R, C]^T (bf16), columns R..Rpad zero; colsum (may be NULL) += column sums of
  * src in fp32 (bias gradients). group > 0: src is [B, group+1, C] and the first row of every

@@ -42,7 +42,19 @@ class vit_preproc_config(Structure):
                 ("image_mean", c_float * 4), ("image_std", c_float * 4)]
 
 
+class vit_qk_norm_config(Structure):
+    _fields_ = [("batch", c_int32), ("seq", c_int32), ("heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+                ("norm", c_int32), ("rot_dim", c_int32), ("interleaved", c_int32), ("rope_len", c_int32),
+                ("positions_per_sample", c_int32), ("dtype", c_int32), ("eps", c_float)]
+
+
+class vit_rel_pos(Structure):
+    _fields_ = [("prefix", c_int32), ("grid_h", c_int32), ("grid_w", c_int32), ("num_buckets", c_int32),
+                ("bucket_of", c_void_p), ("by_bucket", c_void_p), ("bucket_start", c_void_p)]
+
+
 HEAD_LINEAR, HEAD_TANH = 0, 1
+NORM_RMS, NORM_LAYER = 0, 1
 
 # name -> (restype, argtypes): every symbol include/vit_amd.h declares
 SIGNATURES = {
@@ -94,6 +106,13 @@ SIGNATURES = {
     "vit_backward_stage": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_size_t, c_void_p]),
     "vit_sgd_step": (c_int, [c_void_p, c_void_p, c_float, c_void_p]),
+    "vit_qk_norm_rope_fwd": (c_int, [POINTER(vit_qk_norm_config)] + [c_void_p] * 9),
+    "vit_qk_norm_rope_bwd_workspace_bytes": (c_size_t, [POINTER(vit_qk_norm_config)]),
+    "vit_qk_norm_rope_bwd": (c_int, [POINTER(vit_qk_norm_config)] + [c_void_p] * 12 + [c_size_t, c_void_p]),
+    "vit_attention_rel_fwd": (c_int, [POINTER(vit_rel_pos)] + [c_void_p] * 5 + [c_int, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    "vit_attention_rel_bwd_workspace_bytes": (c_size_t, [POINTER(vit_rel_pos), c_int, c_int]),
+    "vit_attention_rel_bwd": (c_int, [POINTER(vit_rel_pos)] + [c_void_p] * 9 + [c_size_t, c_int, c_int, c_int, c_int, c_float,
+                                                                             c_void_p]),
     "vit_head_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                              c_void_p]),
     "vit_pos_embed_interpolate": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),

@@ -1,0 +1,574 @@
+// Backward of attention with a learned relative position bias (attention_rel.hip; bias as in rel_bias.h):
+//
+//   s = scale q.k + bias,  P = exp2(s log2 e - lse),  dP = dO V^T,  delta = rowsum(dO * O),  dS = P * (dP - delta)
+//   dQ = scale dS K,  dK = scale sum_heads dS^T Q,  dV = sum_heads P^T dO,  d_table[b, h] = sum of dS over (sample, i, j) in bucket b
+//
+// Launches, none with atomics (bitwise reproducible):
+//   1 dQ: 32 queries a wave on the lane, keys streamed through LDS. delta from the wave's own rows of dO and O carries the
+//     rounding of O and of the P that made it (about 2^-9), which is nothing beside dQ's own rounding but would stay in the
+//     fp32 sums of dS that make d_table. Rows of the true dS sum to zero (the P of a row sum to 1), so the row sums of the dS
+//     computed with the rounded delta, kept in fp32 beside the products, are its error: delta + sum is written for 2 and 3.
+//   2 dK, dV: 32 keys a wave on the lane, the queries of every head of the group streamed through LDS.
+//   3 bias: one 64 x 64 tile of (query, key) of one head and a range of samples per workgroup. The bias depends on the tile
+//     and not on the sample, and so does the place of dS in its gradient: dS is summed over the samples in registers, and only
+//     the sum is folded by offset (below) -- no scatter in the loop over samples. P and dP are computed again for it
+//     (2 products more), with operands straight from L2 in the MFMA's own layout.
+//   4 offsets: adds the tiles' folded sums per offset in a fixed order; 5 (only with a map) adds the offsets of a bucket.
+//
+// Folding: in a tile, pair (i, j) has linear offset o = i - j in (-64, 64) + tile offset, and the grid offset is
+// dx = o mod gw (class 0: x_i >= dx, no row border between) or that - gw (class 1): 127 diagonals x 2 classes a tile, whatever
+// the grid's width, then three sums for the prefix classes.
+#include "rel_bias.h"
+#include <math.h>
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+enum { MODE_DQ = 0, MODE_DKV = 1 };
+constexpr int TB = 64;              // bias tile
+constexpr int FOLD = 2 * 127 + 3;   // sums a tile leaves
+constexpr int FP = 260;             // their pitch, floats
+
+struct RelBwdArgs {
+    const bf16_t* qkv;
+    const bf16_t* out;
+    const bf16_t* dout;
+    const float* lse;
+    float* delta;  // [B, H, N]
+    bf16_t* dqkv;
+    float* part;   // [splits][H][tiles][tiles][FP]
+    float* doff;   // [H][offsets + 3] (with a map)
+    float* dtable;
+    const int* by_bucket;
+    const int* bucket_start;
+    const int* lengths;
+    RelGeo geo;
+    int B, N, H, HK, IC, splits, tiles;
+    float scale, scale_log2e;
+};
+
+template <int DH>
+struct BGeo {
+    static constexpr int KSTEPS = DH / 16;
+    static constexpr int DB = (DH + 31) / 32;
+    static constexpr int RS = DH * 2 + 16;     // row-read image stride, bytes
+    static constexpr int TS = (DB | 1) * 64;   // transposed-read image stride, bytes
+    static constexpr int CHUNKS = DH / 8;
+};
+
+__device__ __forceinline__ bf16x8 pack8b(const f32x16& p, int s) {
+    bf16x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (bf16_t)p[8 * s + e];
+    return o;
+}
+template <int TS>
+__device__ __forceinline__ bf16x8 tr_frag(const unsigned char* img, int row0, int sk, int d, int tr_key, int tr_col) {
+    const unsigned char* vp = img + (size_t)(row0 + 16 * sk + tr_key) * TS + tr_col + d * 64;
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(vp));
+    const short4v hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(vp + 8 * TS));
+    const short8v both = __builtin_shufflevector(lo, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(bf16x8, both);
+}
+__device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
+    if (!lengths) return N;
+    const int n = lengths[b];
+    return n < 0 ? 0 : n > N ? N : n;
+}
+
+template <int DH, int MODE>
+__global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
+    using G = BGeo<DH>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int IC = a.IC, N = a.N, H = a.H, HK = a.HK;
+    unsigned char* R1 = smem;                        // [IC][RS] K (DQ) / Q (DKV)
+    unsigned char* R2 = R1 + (size_t)IC * G::RS;     // [IC][RS] V (DQ) / dO (DKV)
+    unsigned char* T1 = R2 + (size_t)IC * G::RS;     // [IC][TS] transposed-read image of R1
+    unsigned char* T2 = T1 + (size_t)IC * G::TS;     // of R2 (DKV)
+    float* rowL = (float*)(T2 + (MODE == MODE_DKV ? (size_t)IC * G::TS : 0));  // [IC] (DKV)
+    float* rowD = rowL + (MODE == MODE_DKV ? IC : 0);                          // [IC] (DKV)
+    int* codes = (int*)(rowD + (MODE == MODE_DKV ? IC : 0));                   // [IC]
+    float* T = (float*)(codes + IC);
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nwaves = blockDim.x >> 6;
+    const int r = lane & 31, hi = lane >> 5;
+    const int OH = MODE == MODE_DQ ? H : HK;  // outer heads
+    const int b = blockIdx.x / OH, oh = blockIdx.x - b * OH, group = H / HK;
+    const size_t rs = (size_t)(H + 2 * HK) * DH, os = (size_t)H * DH;
+    const int g = lane >> 4, i16 = lane & 15;
+    const int tr_key = 4 * (g >> 1) + (i16 >> 2);
+    const int tr_col = ((g & 1) * 16 + 4 * (i16 & 3)) * 2;
+    const int nb = sample_length(a.lengths, b, N);
+    const int blk0 = blockIdx.y * nwaves * 32;
+    const int blk1 = min(blk0 + nwaves * 32, N) - 1;
+    const int o0 = blk0 + wave * 32, row = o0 + r;
+    const int orow = row < nb ? row : (nb > 0 ? nb - 1 : 0);
+    const bf16_t* base = a.qkv + (size_t)b * N * rs;
+    const int hk = MODE == MODE_DQ ? oh / group : oh;
+    const bf16_t* kbase = base + (size_t)(H + hk) * DH;
+    const bf16_t* vbase = kbase + (size_t)HK * DH;
+
+    // ---- outer fragments
+    bf16x8 f1[G::KSTEPS], f2[G::KSTEPS];
+    float oL = INFINITY, oD = 0.f;
+    if constexpr (MODE == MODE_DQ) {
+        const size_t at = ((size_t)b * N + orow) * os + (size_t)oh * DH + hi * 8;
+        float d = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < G::KSTEPS; ++ks) {
+            f1[ks] = *(const bf16x8*)(base + (size_t)orow * rs + (size_t)oh * DH + ks * 16 + hi * 8);
+            f2[ks] = *(const bf16x8*)(a.dout + at + ks * 16);
+            const bf16x8 ov = *(const bf16x8*)(a.out + at + ks * 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d = fmaf((float)f2[ks][e], (float)ov[e], d);
+        }
+        oD = d + __shfl_xor(d, 32, 64);
+        if (row < nb) oL = a.lse[((size_t)b * H + oh) * N + row]; else oD = 0.f;
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < G::KSTEPS; ++ks) {
+            f1[ks] = *(const bf16x8*)(kbase + (size_t)orow * rs + ks * 16 + hi * 8);
+            f2[ks] = *(const bf16x8*)(vbase + (size_t)orow * rs + ks * 16 + hi * 8);
+        }
+    }
+    f32x16 acc1[G::DB], acc2[G::DB];  // DQ: acc1 = dQ^T.  DKV: acc1 = dK^T, acc2 = dV^T
+#pragma unroll
+    for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { acc1[d][e] = 0.f; acc2[d][e] = 0.f; }
+
+    const int c0 = rel_code(a.geo, blk0), c1 = rel_code(a.geo, blk1), cmax = rel_code(a.geo, N - 1);
+    const int oc = rel_code(a.geo, row < N ? row : N - 1);
+    const int nheads = MODE == MODE_DQ ? 1 : group;
+    RelTile tile{0.f, 0.f, 0.f, a.geo.prefix};
+    float dsum = 0.f;  // DQ: row sum of dS
+    for (int gh = 0; gh < nheads && nb > 0; ++gh) {
+        const int h = MODE == MODE_DQ ? oh : oh * group + gh;
+        // slice of offsets: DQ lane - row over all keys, DKV row - lane over all queries
+        const int lo = (MODE == MODE_DQ ? c0 - cmax : -c1) + a.geo.center;
+        const int lane_code = MODE == MODE_DQ ? oc + a.geo.center - lo : oc;
+        const int row_add = MODE == MODE_DQ ? 0 : a.geo.center - lo;
+        __syncthreads();
+        rel_expand(a.geo, T, lo, c1 - c0 + cmax + 1, h);
+        if (a.geo.prefix) {
+            tile.e0 = rel_entry(a.geo, a.geo.offsets, h);
+            tile.e1 = rel_entry(a.geo, a.geo.offsets + 1, h);
+            tile.e2 = rel_entry(a.geo, a.geo.offsets + 2, h);
+        }
+        const bf16_t* i1 = MODE == MODE_DQ ? kbase : base + (size_t)h * DH;
+        const bf16_t* i2 = MODE == MODE_DQ ? vbase : a.dout + (size_t)b * N * os + (size_t)h * DH;
+        const size_t s2 = MODE == MODE_DQ ? rs : os;
+        const size_t sat = ((size_t)b * H + h) * N;
+        for (int ic0 = 0; ic0 < nb; ic0 += IC) {
+            int nin = nb - ic0;
+            nin = nin > IC ? IC : (nin + 31) & ~31;
+            __syncthreads();
+            for (int idx = tid; idx < nin * G::CHUNKS; idx += blockDim.x) {
+                const int rr = idx / G::CHUNKS, c = idx - rr * G::CHUNKS;
+                int gr = ic0 + rr;
+                if (gr > nb - 1) gr = nb - 1;  // pad rows re-read the last row; they are masked below
+                const bf16x8 v1 = *(const bf16x8*)(i1 + (size_t)gr * rs + c * 8);
+                const bf16x8 v2 = *(const bf16x8*)(i2 + (size_t)gr * s2 + c * 8);
+                *(bf16x8*)(R1 + (size_t)rr * G::RS + c * 16) = v1;
+                *(bf16x8*)(R2 + (size_t)rr * G::RS + c * 16) = v2;
+                *(bf16x8*)(T1 + (size_t)rr * G::TS + c * 16) = v1;
+                if constexpr (MODE == MODE_DKV) *(bf16x8*)(T2 + (size_t)rr * G::TS + c * 16) = v2;
+            }
+            for (int i = tid; i < nin; i += blockDim.x) {
+                const int gr = ic0 + i;
+                codes[i] = rel_code(a.geo, gr) + row_add;
+                if constexpr (MODE == MODE_DKV) {
+                    rowL[i] = gr < nb ? a.lse[sat + gr] : INFINITY;  // P = exp2(.. - inf) = 0 for pad queries
+                    rowD[i] = gr < nb ? a.delta[sat + gr] : 0.f;
+                }
+            }
+            __syncthreads();
+            for (int t = 0; t < nin >> 5; ++t) {
+                f32x16 s, dp;
+                rel_tile<MODE == MODE_DQ>(s, T, codes + t * 32, lane_code, hi, tile, row, ic0 + t * 32);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+                const unsigned char* p1 = R1 + (size_t)(t * 32 + r) * G::RS + hi * 16;
+                const unsigned char* p2 = R2 + (size_t)(t * 32 + r) * G::RS + hi * 16;
+#pragma unroll
+                for (int ks = 0; ks < G::KSTEPS; ++ks) {
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(p1 + ks * 32), f1[ks], s, 0, 0, 0);
+                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(p2 + ks * 32), f2[ks], dp, 0, 0, 0);
+                }
+                if constexpr (MODE == MODE_DQ) {
+                    const int key0 = ic0 + t * 32;
+                    if (key0 + 32 > nb) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (key0 + (e & 3) + 8 * (e >> 2) + 4 * hi >= nb) s[e] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL);
+                        s[e] = p * (dp[e] - oD);  // dS^T
+                        dsum += s[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const f32x4 L = *(const f32x4*)(rowL + t * 32 + 8 * g4 + 4 * hi);
+                        const f32x4 Dl = *(const f32x4*)(rowD + t * 32 + 8 * g4 + 4 * hi);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int e = g4 * 4 + j;
+                            const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L[j]);
+                            dp[e] = p * (dp[e] - Dl[j]);  // dS
+                            s[e] = p;                     // P
+                        }
+                    }
+                }
+#pragma unroll
+                for (int sk = 0; sk < 2; ++sk) {
+                    const bf16x8 x1 = pack8b(MODE == MODE_DQ ? s : dp, sk);
+#pragma unroll
+                    for (int d = 0; d < G::DB; ++d)
+                        acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<G::TS>(T1, t * 32, sk, d, tr_key, tr_col), x1, acc1[d], 0, 0, 0);
+                    if constexpr (MODE == MODE_DKV) {
+                        const bf16x8 x2 = pack8b(s, sk);
+#pragma unroll
+                        for (int d = 0; d < G::DB; ++d)
+                            acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<G::TS>(T2, t * 32, sk, d, tr_key, tr_col), x2, acc2[d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (MODE == MODE_DQ) {
+        dsum += __shfl_xor(dsum, 32, 64);
+        if (row < N && hi == 0) a.delta[((size_t)b * H + oh) * N + row] = oL < INFINITY ? oD + dsum : 0.f;
+    }
+    // ---- store (rows behind the sample's length: zeros)
+    if (row < N) {
+        const bool live = row < nb;
+        bf16_t* dst = a.dqkv + ((size_t)b * N + row) * rs + (size_t)(MODE == MODE_DQ ? oh : H + oh) * DH;
+#pragma unroll
+        for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const int d0 = d * 32 + 8 * g4 + 4 * hi;
+                if (d0 < DH) {
+                    bf16x4 v, w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[e] = (bf16_t)(live ? acc1[d][g4 * 4 + e] * a.scale : 0.f);
+                        w[e] = (bf16_t)(live ? acc2[d][g4 * 4 + e] : 0.f);
+                    }
+                    *(bf16x4*)(dst + d0) = v;
+                    if constexpr (MODE == MODE_DKV) *(bf16x4*)(dst + (size_t)HK * DH + d0) = w;
+                }
+            }
+    }
+}
+
+// ---- sums of dS over samples, folded by offset. Grid: (tiles * tiles, H, splits); 4 waves, a 32 x 32 quarter each
+template <int DH>
+__global__ __launch_bounds__(256) void attn_rel_bias_grad_kernel(const RelBwdArgs a) {
+    using G = BGeo<DH>;
+    __shared__ float sum[TB][TB + 1];
+    __shared__ float half[2][FOLD];
+    __shared__ float three[4][3];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, hi = lane >> 5;
+    const int N = a.N, H = a.H, HK = a.HK;
+    const int tq = blockIdx.x / a.tiles, tk = blockIdx.x - tq * a.tiles;
+    const int h = blockIdx.y, hk = h / (H / HK);
+    const int iq = (wave >> 1) * 32, ik = (wave & 1) * 32;  // this wave's quarter
+    const int q0 = tq * TB + iq, k0 = tk * TB + ik;
+    const int q = q0 + r;
+    const size_t rs = (size_t)(H + 2 * HK) * DH, os = (size_t)H * DH;
+    const int b0 = (int)((int64_t)a.B * blockIdx.z / a.splits), b1 = (int)((int64_t)a.B * (blockIdx.z + 1) / a.splits);
+
+    // bias of the quarter (register e: key, lane: query)
+    f32x16 bias, acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int k = k0 + (e & 3) + 8 * (e >> 2) + 4 * hi;
+        const bool qp = q < a.geo.prefix, kp = k < a.geo.prefix;
+        const int at = qp ? (kp ? a.geo.offsets + 2 : a.geo.offsets)
+                          : kp ? a.geo.offsets + 1 : rel_code(a.geo, q < N ? q : N - 1) - rel_code(a.geo, k < N ? k : N - 1) + a.geo.center;
+        bias[e] = rel_entry(a.geo, at, h);
+        acc[e] = 0.f;
+    }
+    if (q0 < N && k0 < N) {
+        for (int b = b0; b < b1; ++b) {
+            const int nb = sample_length(a.lengths, b, N);
+            if (q0 >= nb || k0 >= nb) continue;
+            const int qr = q < nb ? q : nb - 1, kr = k0 + r < nb ? k0 + r : nb - 1;
+            const bf16_t* base = a.qkv + (size_t)b * N * rs;
+            const bf16_t* qp = base + (size_t)qr * rs + (size_t)h * DH + hi * 8;
+            const bf16_t* dp_ = a.dout + ((size_t)b * N + qr) * os + (size_t)h * DH + hi * 8;
+            const bf16_t* kp = base + (size_t)kr * rs + (size_t)(H + hk) * DH + hi * 8;
+            const bf16_t* vp = kp + (size_t)HK * DH;
+            const size_t sat = ((size_t)b * H + h) * N;
+            const float L = q < nb ? a.lse[sat + q] : INFINITY;
+            const float D = a.delta[sat + qr];
+            f32x16 s = bias, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < G::KSTEPS; ++ks) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kp + ks * 16), *(const bf16x8*)(qp + ks * 16), s, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(vp + ks * 16), *(const bf16x8*)(dp_ + ks * 16), dp, 0, 0, 0);
+            }
+            if (k0 + 32 > nb) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (k0 + (e & 3) + 8 * (e >> 2) + 4 * hi >= nb) s[e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L);
+                acc[e] += p * (dp[e] - D);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum[iq + r][ik + (e & 3) + 8 * (e >> 2) + 4 * hi] = acc[e];
+    __syncthreads();
+
+    // fold: thread = (diagonal, half of the rows)
+    const int prefix = a.geo.prefix, gw = a.geo.gw;
+    const int tq0 = tq * TB, tk0 = tk * TB;
+    {
+        const int dg = tid & 127, part = tid >> 7;  // diagonal dg: i - j = dg - 63 inside the tile
+        if (dg < 127) {
+            const int o = tq0 - tk0 + dg - 63;  // query token - key token
+            int dx = o % gw;
+            if (dx < 0) dx += gw;
+            float s0 = 0.f, s1 = 0.f;
+            for (int i = part * 32; i < part * 32 + 32; ++i) {
+                const int j = i - (dg - 63);
+                if (j < 0 || j >= TB) continue;
+                const int p = tq0 + i - prefix;
+                if (p < 0 || tk0 + j < prefix || tq0 + i >= N || tk0 + j >= N) continue;
+                const float v = sum[i][j];
+                if (p % gw >= dx) s0 += v; else s1 += v;
+            }
+            half[part][2 * dg] = s0;
+            half[part][2 * dg + 1] = s1;
+        }
+    }
+    if (prefix > 0 && (tq == 0 || tk == 0)) {  // prefix pairs of this tile: 16 columns of a row a thread
+        const int i = tid >> 2, jb = (tid & 3) * 16;
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f;
+        for (int j = jb; j < jb + 16; ++j) {
+            if (tq0 + i >= N || tk0 + j >= N) continue;
+            const bool qp = tq0 + i < prefix, kp = tk0 + j < prefix;
+            const float v = sum[i][j];
+            if (qp && !kp) s0 += v;
+            if (!qp && kp) s1 += v;
+            if (qp && kp) s2 += v;
+        }
+        s0 = wave_sum(s0);
+        s1 = wave_sum(s1);
+        s2 = wave_sum(s2);
+        if (lane == 0) { three[wave][0] = s0; three[wave][1] = s1; three[wave][2] = s2; }
+    } else if (lane == 0) {
+        three[wave][0] = three[wave][1] = three[wave][2] = 0.f;
+    }
+    __syncthreads();
+    float* dst = a.part + ((((size_t)blockIdx.z * H + h) * a.tiles + tq) * a.tiles + tk) * FP;
+    for (int i = tid; i < FOLD; i += 256)
+        dst[i] = i < 254 ? half[0][i] + half[1][i] : (three[0][i - 254] + three[1][i - 254]) + (three[2][i - 254] + three[3][i - 254]);
+}
+
+// ---- per offset: the tiles' folded sums in a fixed order. One wave per (offset index, head): lanes over (split, query tile)
+__global__ __launch_bounds__(256) void attn_rel_offset_kernel(const RelBwdArgs a, float* dst, int stride_h, int stride_o) {
+    const int lane = threadIdx.x & 63;
+    const int idx = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
+    const int offsets = a.geo.offsets;
+    if (idx >= offsets + (a.geo.prefix ? 3 : 0)) return;  // wave-uniform
+    const int gw = a.geo.gw, rows = 2 * gw - 1;
+    const int dyi = idx / rows, dx = idx - dyi * rows - (gw - 1), dy = dyi - (a.geo.center / rows);
+    const int o = dy * gw + dx, cls = dx < 0 ? 1 : 0;
+    float s = 0.f;
+    for (int i = lane; i < a.splits * a.tiles; i += 64) {
+        const int sp = i / a.tiles, tq = i - sp * a.tiles;
+        const float* p = a.part + (((size_t)sp * a.H + h) * a.tiles + tq) * a.tiles * FP;
+        if (idx >= offsets) {
+            for (int tk = 0; tk < a.tiles; ++tk)
+                if (tq == 0 || tk == 0) s += p[(size_t)tk * FP + 254 + idx - offsets];
+        } else {
+            // keys j = i - o of the tile's 64 queries: at most two key tiles
+            const int j0 = tq * TB - o;                      // key of the tile's first query
+            const int t0 = j0 >= 0 ? j0 / TB : -((-j0 + TB - 1) / TB);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int tk = t0 + k;
+                const int dg = o - (tq - tk) * TB + 63;
+                if (tk >= 0 && tk < a.tiles && dg >= 0 && dg < 127) s += p[(size_t)tk * FP + 2 * dg + cls];
+            }
+        }
+    }
+    s = wave_sum(s);
+    if (lane == 0) dst[(size_t)h * stride_h + (size_t)idx * stride_o] = s;
+}
+// ---- per bucket: its offsets' sums in the map's order
+__global__ __launch_bounds__(256) void attn_rel_bucket_kernel(const RelBwdArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int bucket = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
+    if (bucket >= a.geo.num_buckets) return;
+    const int total = a.geo.offsets + (a.geo.prefix ? 3 : 0);
+    float s = 0.f;
+    if (a.geo.bucket_of) {
+        int i0 = a.bucket_start[bucket], i1 = a.bucket_start[bucket + 1];
+        i0 = i0 < 0 ? 0 : i0;
+        i1 = i1 > total ? total : i1;
+        for (int i = i0 + lane; i < i1; i += 64) {
+            const int at = a.by_bucket[i];
+            if (at >= 0 && at < total) s += a.doff[(size_t)h * total + at];
+        }
+    } else if (lane == 0 && bucket < total) {
+        s = a.doff[(size_t)h * total + bucket];
+    }
+    s = wave_sum(s);
+    if (lane == 0) a.dtable[(size_t)bucket * a.H + h] = s;
+}
+
+// waves per workgroup: cover ceil(N / 32) outer tiles with the least padding, at least 4 (staging wants threads)
+int pick_waves_b(int N, int* blocks) {
+    const int n32 = ceil_div(N, 32);
+    int best_w = 4, best_cost = 1 << 30;
+    for (int w = 8; w >= 4; --w) {
+        const int cost = ceil_div(n32, w) * w;
+        if (cost < best_cost) { best_cost = cost; best_w = w; }
+    }
+    *blocks = ceil_div(n32, best_w);
+    return best_w;
+}
+
+template <int DH, int MODE>
+int launch_part(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
+    using G = BGeo<DH>;
+    constexpr int per_row = 2 * G::RS + (MODE == MODE_DKV ? 2 : 1) * G::TS + (MODE == MODE_DKV ? 8 : 0) + 4;
+    constexpr int LDS_MAX = 64 * 1024;
+    int blocks;
+    const int waves = pick_waves_b(a.N, &blocks);
+    int slice = rel_slice_max(pos->prefix, pos->grid_h, pos->grid_w, waves * 32);
+    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
+    const int icmax = LDS_MAX / per_row / 32 * 32;
+    const int npad = (a.N + 31) / 32 * 32;
+    const int nchunks = ceil_div(npad, icmax);
+    a.IC = (ceil_div(npad, nchunks) + 31) / 32 * 32;
+    const size_t lds = (size_t)a.IC * per_row + (size_t)slice * 4;
+    auto kern = attn_rel_bwd_kernel<DH, MODE>;
+    static PerDeviceInt attr_set;
+    std::atomic<int>* as = attr_set.slot();
+    if (!as || !as->load(std::memory_order_relaxed)) {
+        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (as) as->store(1, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(kern, dim3(a.B * (MODE == MODE_DQ ? a.H : a.HK), blocks), dim3(waves * 64), lds, stream, a);
+    VIT_CHECK_HIP(hipGetLastError());
+    return VIT_OK;
+}
+
+// how many workgroups share a bias tile's samples: enough of them to fill the chip, whole samples each
+int bias_splits(int batch, int heads, int tiles, int ncu) {
+    const int64_t have = (int64_t)heads * tiles * tiles;
+    int64_t s = (4LL * ncu + have - 1) / have;
+    if (s > batch) s = batch;
+    return s < 1 ? 1 : (int)s;
+}
+struct Workspace {
+    size_t delta, part, doff, bytes;
+    int tiles, splits;
+};
+int plan_workspace(const vit_rel_pos* pos, int batch, int heads, Workspace* w) {
+    int ncu = 0;
+    VIT_TRY_RC(vit_cu_count(&ncu));
+    const int N = pos->prefix + pos->grid_h * pos->grid_w;
+    w->tiles = ceil_div(N, TB);
+    w->splits = bias_splits(batch, heads, w->tiles, ncu);
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    w->delta = 0;
+    w->part = up((size_t)batch * heads * N * 4);
+    w->doff = w->part + up((size_t)w->splits * heads * w->tiles * w->tiles * FP * 4);
+    w->bytes = w->doff + up((size_t)heads * ((size_t)(2 * pos->grid_h - 1) * (2 * pos->grid_w - 1) + 3) * 4);
+    return VIT_OK;
+}
+
+template <int DH>
+int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
+    VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, stream)));
+    VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, stream)));
+    if (!a.dtable) return VIT_OK;
+    hipLaunchKernelGGL(attn_rel_bias_grad_kernel<DH>, dim3(a.tiles * a.tiles, a.H, a.splits), dim3(256), 0, stream, a);
+    VIT_CHECK_HIP(hipGetLastError());
+    const int total = a.geo.offsets + (a.geo.prefix ? 3 : 0);
+    // without a map, and with nothing in the table behind the offsets, the offset sums are the table's gradient
+    const bool direct = !a.geo.bucket_of && a.geo.num_buckets == total;
+    hipLaunchKernelGGL(attn_rel_offset_kernel, dim3(ceil_div(total, 4), a.H), dim3(256), 0, stream, a, direct ? a.dtable : a.doff,
+                       direct ? 1 : total, direct ? a.H : 1);
+    VIT_CHECK_HIP(hipGetLastError());
+    if (!direct) {
+        hipLaunchKernelGGL(attn_rel_bucket_kernel, dim3(ceil_div(a.geo.num_buckets, 4), a.H), dim3(256), 0, stream, a);
+        VIT_CHECK_HIP(hipGetLastError());
+    }
+    return VIT_OK;
+}
+
+}  // namespace
+
+extern "C" size_t vit_attention_rel_bwd_workspace_bytes(const vit_rel_pos* pos, int batch, int heads) {
+    Workspace w{};
+    if (!pos || batch <= 0 || heads <= 0 || pos->prefix < 0 || pos->grid_h <= 0 || pos->grid_w <= 0 ||
+        (int64_t)pos->grid_h * pos->grid_w > 16384 || plan_workspace(pos, batch, heads, &w) != VIT_OK)
+        return 0;
+    return w.bytes;
+}
+
+extern "C" int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, const float* table, const int32_t* lengths, const void* out,
+                                     const void* d_out, const float* lse, void* dqkv, float* d_table, void* workspace,
+                                     size_t workspace_bytes, int batch, int heads, int kv_heads, int head_dim, float scale, void* stream) {
+    VIT_REQUIRE(qkv && out && d_out && lse && dqkv && workspace, "vit_attention_rel_bwd: null argument");
+    VIT_REQUIRE(batch > 0 && heads > 0 && kv_heads > 0 && heads <= 65535 && (int64_t)batch * heads < (1 << 22),
+                "vit_attention_rel_bwd: empty or too large a problem");
+    VIT_REQUIRE(heads % kv_heads == 0, "vit_attention_rel_bwd: heads %d is not a multiple of kv_heads %d", heads, kv_heads);
+    VIT_REQUIRE(head_dim % 16 == 0 && head_dim >= 16 && head_dim <= 128,
+                "vit_attention_rel_bwd: head_dim must be a multiple of 16 in [16,128], got %d", head_dim);
+    VIT_REQUIRE((((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)d_out | (uintptr_t)dqkv | (uintptr_t)workspace) & 15) == 0,
+                "vit_attention_rel_bwd: tensors must be 16-byte aligned");
+    RelBwdArgs a{};
+    VIT_TRY_RC(rel_make_geo("vit_attention_rel_bwd", pos, table, heads, scale, &a.geo, &a.N));
+    VIT_REQUIRE(!d_table || !pos->bucket_of || (pos->by_bucket && pos->bucket_start),
+                "vit_attention_rel_bwd: the gradient of a mapped table needs the map's inverse");
+    Workspace w{};
+    VIT_TRY_RC(plan_workspace(pos, batch, heads, &w));
+    if (workspace_bytes < w.bytes)
+        return vit_set_error(VIT_E_NOMEM, "vit_attention_rel_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, w.bytes);
+    a.qkv = (const bf16_t*)qkv;
+    a.out = (const bf16_t*)out;
+    a.dout = (const bf16_t*)d_out;
+    a.lse = lse;
+    a.dqkv = (bf16_t*)dqkv;
+    a.delta = (float*)((char*)workspace + w.delta);
+    a.part = (float*)((char*)workspace + w.part);
+    a.doff = (float*)((char*)workspace + w.doff);
+    a.dtable = d_table;
+    a.by_bucket = pos->by_bucket;
+    a.bucket_start = pos->bucket_start;
+    a.lengths = lengths;
+    a.B = batch;
+    a.H = heads;
+    a.HK = kv_heads;
+    a.splits = w.splits;
+    a.tiles = w.tiles;
+    a.scale = scale;
+    a.scale_log2e = scale * LOG2E;
+#define RELB_CASE(DHV) \
+    case DHV: return launch_all<DHV>(a, pos, (hipStream_t)stream);
+    switch (head_dim) {
+        RELB_CASE(16) RELB_CASE(32) RELB_CASE(48) RELB_CASE(64) RELB_CASE(80) RELB_CASE(96) RELB_CASE(112) RELB_CASE(128)
+    }
+#undef RELB_CASE
+    return vit_set_error(VIT_E_INVALID, "vit_attention_rel_bwd: unsupported head_dim %d", head_dim);
+}

@@ -298,3 +298,204 @@ def layer_norm_backward(x, dy, weight, eps: float, d_residual=None):
     _lib.check(_lib.load().vit_layernorm_bwd(x.data_ptr(), dy.data_ptr(), w.data_ptr(), dres, dx.data_ptr(),
                                              dg.data_ptr(), db.data_ptr(), rows, d, float(eps), _stream()))
     return dx, dg, db
+
+
+# --------------------------------------------------------------------------- norms of query / key heads with rotation
+_NORM = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+
+
+def rope_table(grid, rot_dim: int, theta: float | None = None, device="cuda") -> torch.Tensor:
+    """(cos, sin) fp32 ``[grid_h * grid_w, rot_dim / 2, 2]`` for ``qk_norm_rope``: on a ``(grid_h, grid_w)`` grid half of the
+    pairs turn with the row and half with the column (``theta`` 100), on a sequence ``(1, n)`` all of them with the place
+    (``theta`` 10000). Frequencies ``theta ** (-i / pairs)``; the angles are computed in 64 bits."""
+    gh, gw = (int(v) for v in grid)
+    if gh < 1 or gw < 1 or rot_dim < 4 or rot_dim % 4:
+        raise ValueError(f"rope_table: grid {gh} x {gw}, rot_dim {rot_dim}")
+    y = torch.arange(gh, dtype=torch.float64).repeat_interleave(gw)
+    x = torch.arange(gw, dtype=torch.float64).repeat(gh)
+
+    def angles(place, pairs, base):
+        return place[:, None] * base ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+
+    if gh == 1:
+        a = angles(x, rot_dim // 2, 10000.0 if theta is None else float(theta))
+    else:
+        base = 100.0 if theta is None else float(theta)
+        a = torch.cat([angles(y, rot_dim // 4, base), angles(x, rot_dim // 4, base)], dim=-1)
+    return torch.stack([a.cos(), a.sin()], dim=-1).float().to(device)
+
+
+def _same_device(ref: torch.Tensor, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{name} is on {t.device}, qkv on {ref.device}")
+
+
+def _packed_heads(qkv: torch.Tensor, num_heads: int, num_kv_heads: int | None, what: str):
+    """(batch, tokens, key / value heads, head_dim) of a packed [B, N, (H + 2 Hk) dh] projection output"""
+    if qkv.dim() != 3:
+        raise ValueError(f"{what}: qkv must be [batch, tokens, (heads + 2 kv_heads) * head_dim], got {tuple(qkv.shape)}")
+    hk = num_heads if num_kv_heads is None else num_kv_heads
+    if num_heads < 1 or hk < 1 or num_heads % hk:
+        raise ValueError(f"{what}: {num_heads} heads, {hk} key / value heads")
+    b, n, w = qkv.shape
+    if b == 0 or n == 0 or w == 0 or w % (num_heads + 2 * hk):
+        raise ValueError(f"{what}: shape {tuple(qkv.shape)} for {num_heads} + 2 * {hk} heads")
+    return b, n, hk, w // (num_heads + 2 * hk)
+
+
+def _qk_norm_args(qkv, num_heads, num_kv_heads, vectors, eps, rope, positions, interleaved, norm, what):
+    if norm not in _NORM:
+        raise ValueError(f"{what}: unknown norm {norm!r}")
+    b, n, hk, dh = _packed_heads(qkv, num_heads, num_kv_heads, what)
+    _same_device(qkv, rope=rope, positions=positions, **vectors)
+    vec = {}
+    for name, t in vectors.items():
+        if t is not None and t.shape != (dh,):
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({dh},)")
+        vec[name] = _f32(t, name)
+    cfg = _lib.vit_qk_norm_config(b, n, num_heads, hk, dh, _NORM[norm], 0, int(bool(interleaved)), 0, 0, dtype_code(qkv.dtype), float(eps))
+    if rope is not None:
+        if rope.dim() != 3 or rope.shape[2] != 2 or rope.shape[0] == 0:
+            raise ValueError(f"{what}: rope must be [positions, rot_dim / 2, 2], got {tuple(rope.shape)}")
+        rope = _f32(rope, "rope")
+        cfg.rot_dim, cfg.rope_len = 2 * rope.shape[1], rope.shape[0]
+    if positions is not None:
+        if rope is None:
+            raise ValueError(f"{what}: positions without a rope table")
+        if positions.dtype != torch.int32 or positions.shape not in ((n,), (b, n)):
+            raise ValueError(f"{what}: positions must be int32 [{n}] or [{b}, {n}], got {positions.dtype} {tuple(positions.shape)}")
+        positions = _dev(positions, "positions")
+        cfg.positions_per_sample = int(positions.dim() == 2)
+    return cfg, vec, rope, positions
+
+
+def _out_like(ref: torch.Tensor, out, what: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(ref.shape, dtype=ref.dtype, device=ref.device)
+    if out.shape != ref.shape or out.dtype != ref.dtype or out.device != ref.device or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be a contiguous {ref.dtype} tensor of shape {tuple(ref.shape)} on {ref.device}")
+    return out
+
+
+def qk_norm_rope(qkv: torch.Tensor, num_heads: int, q_weight: torch.Tensor, k_weight: torch.Tensor, q_bias=None, k_bias=None,
+                 eps: float = 1e-6, rope: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                 interleaved: bool = False, norm: str = "rms", num_kv_heads: int | None = None, out=None) -> torch.Tensor:
+    """Norm of every query and key head of a packed projection output (``norm``: "rms", or "layer" with optional biases;
+    weights ``[head_dim]`` shared by the heads), then the rotary rotation of the token's position, in one pass: the step
+    between ``linear`` and ``attention`` / ``attention_rel_bias``.
+
+    qkv ``[B, N, (H + 2 Hk) * dh]`` fp32 or bf16, q heads | k heads | v heads; the values pass through. ``rope``: (cos, sin) fp32
+    ``[P, rot_dim / 2, 2]`` (``rope_table``); pairs are ``(i, i + rot_dim / 2)``, or neighbours with ``interleaved``.
+    ``positions``: int32 ``[N]`` or ``[B, N]`` rows of ``rope`` (default: the token's index); one outside ``[0, P)`` leaves its token
+    unturned (-1 for CLS). ``out=qkv`` works in place."""
+    _dev(qkv, "qkv")
+    if norm != "layer" and (q_bias is not None or k_bias is not None):
+        raise ValueError("qk_norm_rope: biases belong to norm='layer'")
+    if out is not None and not qkv.is_contiguous():
+        raise ValueError("qk_norm_rope: out needs a contiguous qkv")
+    qkv = qkv.contiguous()
+    with torch.cuda.device(qkv.device):
+        cfg, vec, rope, positions = _qk_norm_args(qkv, num_heads, num_kv_heads, dict(q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias),
+                                                  eps, rope, positions, interleaved, norm, "qk_norm_rope")
+        out = _out_like(qkv, out, "qk_norm_rope")
+        _lib.check(_lib.load().vit_qk_norm_rope_fwd(cfg, qkv.data_ptr(), *(_ptr(vec[k]) for k in ("q_weight", "k_weight", "q_bias", "k_bias")),
+                                                    _ptr(rope), _ptr(positions), out.data_ptr(), _stream()))
+    return out
+
+
+def qk_norm_rope_backward(qkv: torch.Tensor, d_out: torch.Tensor, num_heads: int, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                          eps: float = 1e-6, rope: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                          interleaved: bool = False, norm: str = "rms", num_kv_heads: int | None = None, out=None):
+    """Gradient of ``qk_norm_rope`` from its INPUT ``qkv`` and the gradient of its output (what ``attention_backward`` returns):
+    ``(dqkv, dq_weight, dk_weight, dq_bias, dk_bias)``, parameter gradients fp32 (biases: ``None`` unless norm is "layer").
+    ``out=d_out`` works in place. Bitwise reproducible."""
+    _dev(qkv, "qkv")
+    _dev(d_out, "d_out")
+    if d_out.shape != qkv.shape or d_out.dtype != qkv.dtype:
+        raise ValueError(f"qk_norm_rope_backward: d_out {d_out.dtype} {tuple(d_out.shape)} for qkv {qkv.dtype} {tuple(qkv.shape)}")
+    _same_device(qkv, d_out=d_out)
+    if out is not None and not d_out.is_contiguous():
+        raise ValueError("qk_norm_rope_backward: out needs a contiguous d_out")
+    qkv, d_out = qkv.contiguous(), d_out.contiguous()
+    with torch.cuda.device(qkv.device):
+        cfg, vec, rope, positions = _qk_norm_args(qkv, num_heads, num_kv_heads, dict(q_weight=q_weight, k_weight=k_weight),
+                                                  eps, rope, positions, interleaved, norm, "qk_norm_rope_backward")
+        out = _out_like(d_out, out, "qk_norm_rope_backward")
+        lib = _lib.load()
+        sums = torch.empty(4 if norm == "layer" else 2, cfg.head_dim, dtype=torch.float32, device=qkv.device)
+        need = lib.vit_qk_norm_rope_bwd_workspace_bytes(cfg)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=qkv.device)
+        grads = [s for s in sums] + [None] * (4 - len(sums))
+        _lib.check(lib.vit_qk_norm_rope_bwd(cfg, qkv.data_ptr(), d_out.data_ptr(), vec["q_weight"].data_ptr(), vec["k_weight"].data_ptr(),
+                                            _ptr(rope), _ptr(positions), out.data_ptr(), *(_ptr(g) for g in grads), ws.data_ptr(), need,
+                                            _stream()))
+    return (out, *grads)
+
+
+# --------------------------------------------------------------------------- attention with a relative position bias
+def _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, what):
+    b, n, hk, dh = _packed_heads(qkv, num_heads, num_kv_heads, what)
+    if n != buckets.seq:
+        raise ValueError(f"{what}: qkv has {n} tokens, the buckets are for {buckets.seq}")
+    if table.shape != (buckets.num_buckets, num_heads):
+        raise ValueError(f"{what}: table has shape {tuple(table.shape)}, expected ({buckets.num_buckets}, {num_heads})")
+    _same_device(qkv, table=table, lengths=lengths, buckets=buckets.bucket_of)
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or lengths.shape != (b,):
+            raise ValueError(f"{what}: lengths must be int32 [{b}], got {lengths.dtype} {tuple(lengths.shape)}")
+        lengths = _dev(lengths, "lengths")
+    return b, n, hk, dh, _f32(table, "table"), lengths, dh ** -0.5 if scale is None else float(scale)
+
+
+def attention_rel_bias(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, buckets, lengths: torch.Tensor | None = None,
+                       num_kv_heads: int | None = None, scale: float | None = None) -> torch.Tensor:
+    """``attention`` with a learned relative position bias: softmax(scale Q K^T + table[bucket(i, j), head]) V.
+
+    qkv ``[B, N, (H + 2 Hk) * dh]`` fp32 or bf16 -> ``[B, N, H * dh]``; ``table`` ``[num_buckets, H]`` (entries below -1e30 mask their
+    pairs; a query left without a key gives zeros); ``buckets``: ``rel_pos.RelPosBuckets``; ``lengths``: int32 ``[B]``, tokens in use
+    (rows behind give zeros); ``scale`` defaults to ``dh ** -0.5``."""
+    qkv = _dev(qkv, "qkv")
+    with torch.cuda.device(qkv.device):
+        b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias")
+        out = torch.empty(b, n, num_heads * dh, dtype=qkv.dtype, device=qkv.device)
+        _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(), None,
+                                                     b, num_heads, hk, dh, scale, dtype_code(qkv.dtype), _stream()))
+    return out
+
+
+def attention_rel_bias_train(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, buckets, lengths: torch.Tensor | None = None,
+                             num_kv_heads: int | None = None, scale: float | None = None):
+    """``attention_rel_bias`` (bf16) that also returns what its backward needs: ``(out, saved)``, ``saved`` the base-2 log-sum-exp of
+    every row ``[B, H, N]`` (+inf where a query has no key)."""
+    qkv = _bf16(qkv, "qkv")
+    with torch.cuda.device(qkv.device):
+        b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias_train")
+        out = torch.empty(b, n, num_heads * dh, dtype=qkv.dtype, device=qkv.device)
+        lse = torch.empty(b, num_heads, n, dtype=torch.float32, device=qkv.device)
+        _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(),
+                                                     lse.data_ptr(), b, num_heads, hk, dh, scale, _lib.VIT_BF16, _stream()))
+    return out, lse
+
+
+def attention_rel_bias_backward(qkv: torch.Tensor, out: torch.Tensor, d_out: torch.Tensor, saved, num_heads: int, table: torch.Tensor,
+                                buckets, lengths: torch.Tensor | None = None, num_kv_heads: int | None = None, scale: float | None = None):
+    """Gradient of ``attention_rel_bias`` from ``attention_rel_bias_train``'s ``(out, saved)`` and the gradient of ``out``:
+    ``(dqkv bf16, d_table fp32 [num_buckets, H])``. The other arguments as in the forward. Bitwise reproducible."""
+    qkv, out, d_out = _bf16(qkv, "qkv"), _bf16(out, "out"), _bf16(d_out, "d_out")
+    with torch.cuda.device(qkv.device):
+        b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias_backward")
+        for name, t, shape, dt in (("out", out, (b, n, num_heads * dh), torch.bfloat16), ("d_out", d_out, (b, n, num_heads * dh), torch.bfloat16),
+                                   ("saved", saved, (b, num_heads, n), torch.float32)):
+            if t.shape != shape or t.dtype != dt or t.device != qkv.device or not t.is_contiguous():
+                raise ValueError(f"attention_rel_bias_backward: {name} must be {dt} {shape} on {qkv.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        lib = _lib.load()
+        c = buckets._c()
+        need = lib.vit_attention_rel_bwd_workspace_bytes(c, b, num_heads)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=qkv.device)
+        dqkv = torch.empty_like(qkv)
+        d_table = torch.empty(buckets.num_buckets, num_heads, dtype=torch.float32, device=qkv.device)
+        _lib.check(lib.vit_attention_rel_bwd(c, qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(),
+                                             d_out.data_ptr(), saved.data_ptr(), dqkv.data_ptr(), d_table.data_ptr(), ws.data_ptr(), need,
+                                             b, num_heads, hk, dh, scale, _stream()))
+    return dqkv, d_table
