@@ -42,25 +42,6 @@ __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
     return n < 0 ? 0 : n > N ? N : n;
 }
 
-// ---- what both element types share: the expansion of this block's slice and its codes
-struct RelBlock {
-    int lo;         // first offset index of the slice
-    RelTile tile;
-};
-__device__ __forceinline__ RelBlock rel_query_block(const RelGeo& g, float* T, int first, int last, int head) {
-    RelBlock r;
-    const int c0 = rel_code(g, first), c1 = rel_code(g, last), cmax = rel_code(g, g.prefix + g.grid - 1);
-    r.lo = c0 - cmax + g.center;
-    rel_expand(g, T, r.lo, c1 - c0 + cmax + 1, head);
-    r.tile = {0.f, 0.f, 0.f, g.prefix};
-    if (g.prefix) {
-        r.tile.e0 = rel_entry(g, g.offsets, head);
-        r.tile.e1 = rel_entry(g, g.offsets + 1, head);
-        r.tile.e2 = rel_entry(g, g.offsets + 2, head);
-    }
-    return r;
-}
-
 template <int DH>
 __global__ __launch_bounds__(512) void attention_rel_bf16_kernel(const RelFwdArgs a) {
     using G = RGeo<DH>;
@@ -90,8 +71,9 @@ __global__ __launch_bounds__(512) void attention_rel_bf16_kernel(const RelFwdArg
     for (int ks = 0; ks < G::KSTEPS; ++ks) qf[ks] = *(const bf16x8*)(base + (size_t)qrow * rs + (size_t)h * DH + ks * 16 + hi * 8);
 
     const int blk1 = blk0 + nwaves * 32 - 1;
-    const RelBlock rb = rel_query_block(a.geo, T, blk0, blk1 < N ? blk1 : N - 1, h);
-    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - rb.lo;
+    const RelSlice sl(a.geo, blk0, blk1 < N ? blk1 : N - 1, true);
+    rel_expand(a.geo, T, sl.lo, sl.n, h);
+    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - sl.lo;
 
     f32x16 o[G::DB];
 #pragma unroll
@@ -122,7 +104,7 @@ __global__ __launch_bounds__(512) void attention_rel_bf16_kernel(const RelFwdArg
         for (int t = 0; t < nkeys >> 5; ++t) {
             const int key0 = kc0 + t * 32;
             f32x16 s;
-            rel_tile<true>(s, T, codes + t * 32, qcode, hi, rb.tile, q, key0);
+            rel_tile<true>(s, T, codes + t * 32, qcode, hi, a.geo.prefix, sl.n, q, key0);
             const unsigned char* kp = Kl + (size_t)(t * 32 + r) * G::KS + hi * 16;
 #pragma unroll
             for (int ks = 0; ks < G::KSTEPS; ++ks)
@@ -222,8 +204,9 @@ __global__ __launch_bounds__(512) void attention_rel_f32_kernel(const RelFwdArgs
     for (int t = 0; t < DH / 2; ++t) qf[t] = base[(size_t)qrow * rs + (size_t)h * DH + 2 * t + hi];
 
     const int blk1 = blk0 + nwaves * 32 - 1;
-    const RelBlock rb = rel_query_block(a.geo, T, blk0, blk1 < N ? blk1 : N - 1, h);
-    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - rb.lo;
+    const RelSlice sl(a.geo, blk0, blk1 < N ? blk1 : N - 1, true);
+    rel_expand(a.geo, T, sl.lo, sl.n, h);
+    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - sl.lo;
 
     f32x16 o[DB];
 #pragma unroll
@@ -253,7 +236,7 @@ __global__ __launch_bounds__(512) void attention_rel_f32_kernel(const RelFwdArgs
         for (int t = 0; t < nkeys >> 5; ++t) {
             const int key0 = kc0 + t * 32;
             f32x16 s;
-            rel_tile<true>(s, T, codes + t * 32, qcode, hi, rb.tile, q, key0);
+            rel_tile<true>(s, T, codes + t * 32, qcode, hi, a.geo.prefix, sl.n, q, key0);
             const float* kp = Kl + (size_t)(t * 32 + r) * KSF + hi;
 #pragma unroll
             for (int kk = 0; kk < DH / 2; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kp[2 * kk], qf[kk], s, 0, 0, 0);
@@ -329,9 +312,7 @@ int launch_rel(RelFwdArgs a, const vit_rel_pos* pos, int batch, int dtype, hipSt
     int qblocks;
     const int waves = pick_waves(a.N, &qblocks);
     const int per_key = dtype == VIT_BF16 ? RGeo<DH>::KS + RGeo<DH>::VS + 4 : (DH + 1 + (DH + 31) / 32 * 32 + 1) * 4;
-    a.slice = rel_slice_max(pos->prefix, pos->grid_h, pos->grid_w, waves * 32);
-    const int all = (2 * pos->grid_h - 1) * (2 * pos->grid_w - 1);
-    if (a.slice > all) a.slice = all;
+    a.slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
     VIT_REQUIRE(a.slice <= kRelSliceCap, "attention_rel: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, a.slice, kRelSliceCap);
     int KC = 80 * 1024 / per_key / 32 * 32;
     const int npad = (a.N + 31) / 32 * 32;
@@ -352,6 +333,11 @@ int launch_rel(RelFwdArgs a, const vit_rel_pos* pos, int batch, int dtype, hipSt
 }
 
 }  // namespace
+
+// persistent LDS-DMA ring for head_dim 64 and whole sequences (attention_rel_dh64.hip)
+bool attention_rel_dh64_eligible(const vit_rel_pos* pos, int batch, int heads, int kv_heads);
+int launch_attention_rel_dh64(const vit_rel_pos* pos, const RelGeo& geo, const void* qkv, void* out, float* lse, int batch, int heads, int kv_heads,
+                              float scale, hipStream_t stream);
 
 int rel_make_geo(const char* who, const vit_rel_pos* pos, const float* table, int heads, float scale, RelGeo* out, int* seq) {
     VIT_REQUIRE(pos && table, "%s: null argument", who);
@@ -388,6 +374,8 @@ extern "C" int vit_attention_rel_fwd(const vit_rel_pos* pos, const void* qkv, co
     a.H = heads;
     a.HK = kv_heads;
     a.scale_log2e = scale * LOG2E;
+    if (dtype == VIT_BF16 && head_dim == 64 && !lengths && attention_rel_dh64_eligible(pos, batch, heads, kv_heads))
+        return launch_attention_rel_dh64(pos, a.geo, qkv, out, lse, batch, heads, kv_heads, scale, (hipStream_t)stream);
 #define REL_CASE(DHV) \
     case DHV: return launch_rel<DHV>(a, pos, batch, dtype, (hipStream_t)stream);
     switch (head_dim) {

@@ -139,24 +139,16 @@ __global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) { acc1[d][e] = 0.f; acc2[d][e] = 0.f; }
 
-    const int c0 = rel_code(a.geo, blk0), c1 = rel_code(a.geo, blk1), cmax = rel_code(a.geo, N - 1);
+    const RelSlice sl(a.geo, blk0, blk1, MODE == MODE_DQ);  // over all keys / all queries
     const int oc = rel_code(a.geo, row < N ? row : N - 1);
     const int nheads = MODE == MODE_DQ ? 1 : group;
-    RelTile tile{0.f, 0.f, 0.f, a.geo.prefix};
     float dsum = 0.f;  // DQ: row sum of dS
     for (int gh = 0; gh < nheads && nb > 0; ++gh) {
         const int h = MODE == MODE_DQ ? oh : oh * group + gh;
-        // slice of offsets: DQ lane - row over all keys, DKV row - lane over all queries
-        const int lo = (MODE == MODE_DQ ? c0 - cmax : -c1) + a.geo.center;
-        const int lane_code = MODE == MODE_DQ ? oc + a.geo.center - lo : oc;
-        const int row_add = MODE == MODE_DQ ? 0 : a.geo.center - lo;
+        const int lane_code = MODE == MODE_DQ ? oc + a.geo.center - sl.lo : oc;
+        const int row_add = MODE == MODE_DQ ? 0 : a.geo.center - sl.lo;
         __syncthreads();
-        rel_expand(a.geo, T, lo, c1 - c0 + cmax + 1, h);
-        if (a.geo.prefix) {
-            tile.e0 = rel_entry(a.geo, a.geo.offsets, h);
-            tile.e1 = rel_entry(a.geo, a.geo.offsets + 1, h);
-            tile.e2 = rel_entry(a.geo, a.geo.offsets + 2, h);
-        }
+        rel_expand(a.geo, T, sl.lo, sl.n, h);
         const bf16_t* i1 = MODE == MODE_DQ ? kbase : base + (size_t)h * DH;
         const bf16_t* i2 = MODE == MODE_DQ ? vbase : a.dout + (size_t)b * N * os + (size_t)h * DH;
         const size_t s2 = MODE == MODE_DQ ? rs : os;
@@ -187,7 +179,7 @@ __global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
             __syncthreads();
             for (int t = 0; t < nin >> 5; ++t) {
                 f32x16 s, dp;
-                rel_tile<MODE == MODE_DQ>(s, T, codes + t * 32, lane_code, hi, tile, row, ic0 + t * 32);
+                rel_tile<MODE == MODE_DQ>(s, T, codes + t * 32, lane_code, hi, a.geo.prefix, sl.n, row, ic0 + t * 32);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dp[e] = 0.f;
                 const unsigned char* p1 = R1 + (size_t)(t * 32 + r) * G::RS + hi * 16;
@@ -452,7 +444,7 @@ int launch_part(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
     constexpr int LDS_MAX = 64 * 1024;
     int blocks;
     const int waves = pick_waves_b(a.N, &blocks);
-    int slice = rel_slice_max(pos->prefix, pos->grid_h, pos->grid_w, waves * 32);
+    int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
     VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     const int icmax = LDS_MAX / per_row / 32 * 32;
     const int npad = (a.N + 31) / 32 * 32;

@@ -303,20 +303,37 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(const QkArgs a) {
     }
 }
 
-// column sums of the blocks' partial rows [blocks][ns * dh]: 16 columns a block, 16 row groups, joined in a fixed order
-__global__ __launch_bounds__(256) void qk_norm_rope_sum_kernel(const float* __restrict__ part, int blocks, int dh, int ns, float* dwq,
-                                                               float* dwk, float* dbq, float* dbk) {
-    __shared__ float red[16][17];
+// column sums of the blocks' partial rows [blocks][ns * dh]: 16 columns a block, 64 row groups with their loads in flight
+// together, joined in a fixed order
+__global__ __launch_bounds__(1024) void qk_norm_rope_sum_kernel(const float* __restrict__ part, int blocks, int dh, int ns, float* dwq,
+                                                                float* dwk, float* dbq, float* dbk) {
+    __shared__ float red[64][17];
     const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
     const int col = blockIdx.x * 16 + c, cols = ns * dh;  // dh is a multiple of 16: every column exists
     float s = 0.f;
-    for (int i = g; i < blocks; i += 16) s += part[(size_t)i * cols + col];
+    for (int i0 = 0; i0 < blocks; i0 += 64 * 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k * 64 + g;
+            v[k] = i < blocks ? part[(size_t)i * cols + col] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += v[k];
+    }
     red[g][c] = s;
     __syncthreads();
-    if (g == 0) {
-        float v = 0.f;
+    if (g < 8) {
+        s = red[g][c];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v += red[k][c];
+        for (int k = 1; k < 8; ++k) s += red[g + 8 * k][c];
+        red[g][c] = s;  // (each of these rows is read by its own thread alone above)
+    }
+    __syncthreads();
+    if (g == 0) {
+        float v = red[0][c];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v += red[k][c];
         const int which = col / dh, d = col - which * dh;
         float* dst = which == 0 ? dwq : which == 1 ? dwk : which == 2 ? dbq : dbk;
         if (dst) dst[d] = v;
@@ -452,7 +469,7 @@ extern "C" int vit_qk_norm_rope_bwd(const vit_qk_norm_config* cfg, const void* q
     launch_any<true>(a, cfg, blocks, (hipStream_t)stream);
     VIT_CHECK_HIP(hipGetLastError());
     const int ns = cfg->norm == VIT_NORM_LAYER ? 4 : 2;
-    hipLaunchKernelGGL(qk_norm_rope_sum_kernel, dim3(ns * cfg->head_dim / 16), dim3(256), 0, (hipStream_t)stream, a.part, blocks,
+    hipLaunchKernelGGL(qk_norm_rope_sum_kernel, dim3(ns * cfg->head_dim / 16), dim3(1024), 0, (hipStream_t)stream, a.part, blocks,
                        cfg->head_dim, ns, dq_weight, dk_weight, dq_bias, dk_bias);
     VIT_CHECK_HIP(hipGetLastError());
     return VIT_OK;

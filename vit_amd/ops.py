@@ -325,10 +325,30 @@ def rope_table(grid, rot_dim: int, theta: float | None = None, device="cuda") ->
     return torch.stack([a.cos(), a.sin()], dim=-1).float().to(device)
 
 
-def _same_device(ref: torch.Tensor, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, qkv on {ref.device}")
+def _elsewhere(t: torch.Tensor) -> bool:
+    """whether ``t`` lives on another device than the current one (the calls below then enter it)"""
+    return t.is_cuda and t.device.index != torch.cuda.current_device()
+
+
+def _raw_stream(t: torch.Tensor) -> int:
+    """The current stream of ``t``'s device as a handle: what ``torch.cuda.current_stream().cuda_stream`` gives, without building
+    the Stream object (2.6 us of a 5 us call)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _vec(t, name: str, n: int, ref: torch.Tensor, what: str):
+    """an fp32 contiguous vector of ``n`` on ``ref``'s device, or None"""
+    if t is None:
+        return None
+    if t.shape != (n,):
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({n},)")
+    return _near(t, name, ref).float().contiguous()
+
+
+def _near(t: torch.Tensor, name: str, ref: torch.Tensor) -> torch.Tensor:
+    if t.device != ref.device:
+        raise ValueError(f"{name} is on {t.device}, qkv on {ref.device}")
+    return t
 
 
 def _packed_heads(qkv: torch.Tensor, num_heads: int, num_kv_heads: int | None, what: str):
@@ -344,35 +364,31 @@ def _packed_heads(qkv: torch.Tensor, num_heads: int, num_kv_heads: int | None, w
     return b, n, hk, w // (num_heads + 2 * hk)
 
 
-def _qk_norm_args(qkv, num_heads, num_kv_heads, vectors, eps, rope, positions, interleaved, norm, what):
+def _qk_norm_args(qkv, num_heads, num_kv_heads, eps, rope, positions, interleaved, norm, what):
     if norm not in _NORM:
         raise ValueError(f"{what}: unknown norm {norm!r}")
     b, n, hk, dh = _packed_heads(qkv, num_heads, num_kv_heads, what)
-    _same_device(qkv, rope=rope, positions=positions, **vectors)
-    vec = {}
-    for name, t in vectors.items():
-        if t is not None and t.shape != (dh,):
-            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({dh},)")
-        vec[name] = _f32(t, name)
-    cfg = _lib.vit_qk_norm_config(b, n, num_heads, hk, dh, _NORM[norm], 0, int(bool(interleaved)), 0, 0, dtype_code(qkv.dtype), float(eps))
+    rot_dim = rope_len = per_sample = 0
     if rope is not None:
         if rope.dim() != 3 or rope.shape[2] != 2 or rope.shape[0] == 0:
             raise ValueError(f"{what}: rope must be [positions, rot_dim / 2, 2], got {tuple(rope.shape)}")
-        rope = _f32(rope, "rope")
-        cfg.rot_dim, cfg.rope_len = 2 * rope.shape[1], rope.shape[0]
+        rope = _near(rope, "rope", qkv).float().contiguous()
+        rope_len, rot_dim = rope.shape[0], 2 * rope.shape[1]
     if positions is not None:
         if rope is None:
             raise ValueError(f"{what}: positions without a rope table")
-        if positions.dtype != torch.int32 or positions.shape not in ((n,), (b, n)):
+        per_sample = positions.dim() == 2
+        if positions.dtype != torch.int32 or positions.shape != ((b, n) if per_sample else (n,)):
             raise ValueError(f"{what}: positions must be int32 [{n}] or [{b}, {n}], got {positions.dtype} {tuple(positions.shape)}")
-        positions = _dev(positions, "positions")
-        cfg.positions_per_sample = int(positions.dim() == 2)
-    return cfg, vec, rope, positions
+        positions = _near(positions, "positions", qkv).contiguous()
+    cfg = _lib.vit_qk_norm_config(b, n, num_heads, hk, dh, _NORM[norm], rot_dim, bool(interleaved), rope_len, per_sample,
+                                  dtype_code(qkv.dtype), eps)
+    return cfg, dh, rope, positions
 
 
 def _out_like(ref: torch.Tensor, out, what: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(ref.shape, dtype=ref.dtype, device=ref.device)
+        return torch.empty_like(ref)
     if out.shape != ref.shape or out.dtype != ref.dtype or out.device != ref.device or not out.is_contiguous():
         raise ValueError(f"{what}: out must be a contiguous {ref.dtype} tensor of shape {tuple(ref.shape)} on {ref.device}")
     return out
@@ -389,18 +405,22 @@ def qk_norm_rope(qkv: torch.Tensor, num_heads: int, q_weight: torch.Tensor, k_we
     ``[P, rot_dim / 2, 2]`` (``rope_table``); pairs are ``(i, i + rot_dim / 2)``, or neighbours with ``interleaved``.
     ``positions``: int32 ``[N]`` or ``[B, N]`` rows of ``rope`` (default: the token's index); one outside ``[0, P)`` leaves its token
     unturned (-1 for CLS). ``out=qkv`` works in place."""
-    _dev(qkv, "qkv")
+    if _elsewhere(qkv):
+        with torch.cuda.device(qkv.device):
+            return qk_norm_rope(qkv, num_heads, q_weight, k_weight, q_bias, k_bias, eps, rope, positions, interleaved, norm, num_kv_heads, out)
     if norm != "layer" and (q_bias is not None or k_bias is not None):
         raise ValueError("qk_norm_rope: biases belong to norm='layer'")
     if out is not None and not qkv.is_contiguous():
         raise ValueError("qk_norm_rope: out needs a contiguous qkv")
-    qkv = qkv.contiguous()
-    with torch.cuda.device(qkv.device):
-        cfg, vec, rope, positions = _qk_norm_args(qkv, num_heads, num_kv_heads, dict(q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias),
-                                                  eps, rope, positions, interleaved, norm, "qk_norm_rope")
-        out = _out_like(qkv, out, "qk_norm_rope")
-        _lib.check(_lib.load().vit_qk_norm_rope_fwd(cfg, qkv.data_ptr(), *(_ptr(vec[k]) for k in ("q_weight", "k_weight", "q_bias", "k_bias")),
-                                                    _ptr(rope), _ptr(positions), out.data_ptr(), _stream()))
+    what = "qk_norm_rope"
+    qkv = _dev(qkv, "qkv")
+    cfg, dh, rope, positions = _qk_norm_args(qkv, num_heads, num_kv_heads, eps, rope, positions, interleaved, norm, what)
+    # (named: a converted copy lives until the launch is enqueued)
+    qw, kw = _vec(q_weight, "q_weight", dh, qkv, what), _vec(k_weight, "k_weight", dh, qkv, what)
+    qb, kb = _vec(q_bias, "q_bias", dh, qkv, what), _vec(k_bias, "k_bias", dh, qkv, what)
+    out = _out_like(qkv, out, what)
+    _lib.check(_lib.load().vit_qk_norm_rope_fwd(cfg, qkv.data_ptr(), qw.data_ptr(), kw.data_ptr(), _ptr(qb), _ptr(kb), _ptr(rope),
+                                                _ptr(positions), out.data_ptr(), _raw_stream(qkv)))
     return out
 
 
@@ -410,26 +430,25 @@ def qk_norm_rope_backward(qkv: torch.Tensor, d_out: torch.Tensor, num_heads: int
     """Gradient of ``qk_norm_rope`` from its INPUT ``qkv`` and the gradient of its output (what ``attention_backward`` returns):
     ``(dqkv, dq_weight, dk_weight, dq_bias, dk_bias)``, parameter gradients fp32 (biases: ``None`` unless norm is "layer").
     ``out=d_out`` works in place. Bitwise reproducible."""
-    _dev(qkv, "qkv")
-    _dev(d_out, "d_out")
-    if d_out.shape != qkv.shape or d_out.dtype != qkv.dtype:
-        raise ValueError(f"qk_norm_rope_backward: d_out {d_out.dtype} {tuple(d_out.shape)} for qkv {qkv.dtype} {tuple(qkv.shape)}")
-    _same_device(qkv, d_out=d_out)
+    if _elsewhere(qkv):
+        with torch.cuda.device(qkv.device):
+            return qk_norm_rope_backward(qkv, d_out, num_heads, q_weight, k_weight, eps, rope, positions, interleaved, norm, num_kv_heads, out)
+    what = "qk_norm_rope_backward"
     if out is not None and not d_out.is_contiguous():
-        raise ValueError("qk_norm_rope_backward: out needs a contiguous d_out")
-    qkv, d_out = qkv.contiguous(), d_out.contiguous()
-    with torch.cuda.device(qkv.device):
-        cfg, vec, rope, positions = _qk_norm_args(qkv, num_heads, num_kv_heads, dict(q_weight=q_weight, k_weight=k_weight),
-                                                  eps, rope, positions, interleaved, norm, "qk_norm_rope_backward")
-        out = _out_like(d_out, out, "qk_norm_rope_backward")
-        lib = _lib.load()
-        sums = torch.empty(4 if norm == "layer" else 2, cfg.head_dim, dtype=torch.float32, device=qkv.device)
-        need = lib.vit_qk_norm_rope_bwd_workspace_bytes(cfg)
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=qkv.device)
-        grads = [s for s in sums] + [None] * (4 - len(sums))
-        _lib.check(lib.vit_qk_norm_rope_bwd(cfg, qkv.data_ptr(), d_out.data_ptr(), vec["q_weight"].data_ptr(), vec["k_weight"].data_ptr(),
-                                            _ptr(rope), _ptr(positions), out.data_ptr(), *(_ptr(g) for g in grads), ws.data_ptr(), need,
-                                            _stream()))
+        raise ValueError(f"{what}: out needs a contiguous d_out")
+    qkv, d_out = _dev(qkv, "qkv"), _near(_dev(d_out, "d_out"), "d_out", qkv)
+    if d_out.shape != qkv.shape or d_out.dtype != qkv.dtype:
+        raise ValueError(f"{what}: d_out {d_out.dtype} {tuple(d_out.shape)} for qkv {qkv.dtype} {tuple(qkv.shape)}")
+    cfg, dh, rope, positions = _qk_norm_args(qkv, num_heads, num_kv_heads, eps, rope, positions, interleaved, norm, what)
+    qw, kw = _vec(q_weight, "q_weight", dh, qkv, what), _vec(k_weight, "k_weight", dh, qkv, what)
+    out = _out_like(d_out, out, what)
+    lib = _lib.load()
+    sums = torch.empty((4 if norm == "layer" else 2, dh), dtype=torch.float32, device=qkv.device)
+    need = lib.vit_qk_norm_rope_bwd_workspace_bytes(cfg)
+    ws = torch.empty((need,), dtype=torch.uint8, device=qkv.device)
+    grads = [*sums.unbind()] + [None] * (4 - sums.shape[0])
+    _lib.check(lib.vit_qk_norm_rope_bwd(cfg, qkv.data_ptr(), d_out.data_ptr(), qw.data_ptr(), kw.data_ptr(), _ptr(rope), _ptr(positions),
+                                        out.data_ptr(), *map(_ptr, grads), ws.data_ptr(), need, _raw_stream(qkv)))
     return (out, *grads)
 
 
@@ -440,12 +459,14 @@ def _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, what
         raise ValueError(f"{what}: qkv has {n} tokens, the buckets are for {buckets.seq}")
     if table.shape != (buckets.num_buckets, num_heads):
         raise ValueError(f"{what}: table has shape {tuple(table.shape)}, expected ({buckets.num_buckets}, {num_heads})")
-    _same_device(qkv, table=table, lengths=lengths, buckets=buckets.bucket_of)
+    table = _near(table, "table", qkv).float().contiguous()
+    if buckets.bucket_of is not None:
+        _near(buckets.bucket_of, "buckets", qkv)
     if lengths is not None:
         if lengths.dtype != torch.int32 or lengths.shape != (b,):
             raise ValueError(f"{what}: lengths must be int32 [{b}], got {lengths.dtype} {tuple(lengths.shape)}")
-        lengths = _dev(lengths, "lengths")
-    return b, n, hk, dh, _f32(table, "table"), lengths, dh ** -0.5 if scale is None else float(scale)
+        lengths = _near(lengths, "lengths", qkv).contiguous()
+    return b, n, hk, dh, table, lengths, dh ** -0.5 if scale is None else scale
 
 
 def attention_rel_bias(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, buckets, lengths: torch.Tensor | None = None,
@@ -455,12 +476,14 @@ def attention_rel_bias(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, b
     qkv ``[B, N, (H + 2 Hk) * dh]`` fp32 or bf16 -> ``[B, N, H * dh]``; ``table`` ``[num_buckets, H]`` (entries below -1e30 mask their
     pairs; a query left without a key gives zeros); ``buckets``: ``rel_pos.RelPosBuckets``; ``lengths``: int32 ``[B]``, tokens in use
     (rows behind give zeros); ``scale`` defaults to ``dh ** -0.5``."""
+    if _elsewhere(qkv):
+        with torch.cuda.device(qkv.device):
+            return attention_rel_bias(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale)
     qkv = _dev(qkv, "qkv")
-    with torch.cuda.device(qkv.device):
-        b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias")
-        out = torch.empty(b, n, num_heads * dh, dtype=qkv.dtype, device=qkv.device)
-        _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(), None,
-                                                     b, num_heads, hk, dh, scale, dtype_code(qkv.dtype), _stream()))
+    b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias")
+    out = torch.empty((b, n, num_heads * dh), dtype=qkv.dtype, device=qkv.device)
+    _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(), None,
+                                                 b, num_heads, hk, dh, scale, dtype_code(qkv.dtype), _raw_stream(qkv)))
     return out
 
 
@@ -468,13 +491,15 @@ def attention_rel_bias_train(qkv: torch.Tensor, num_heads: int, table: torch.Ten
                              num_kv_heads: int | None = None, scale: float | None = None):
     """``attention_rel_bias`` (bf16) that also returns what its backward needs: ``(out, saved)``, ``saved`` the base-2 log-sum-exp of
     every row ``[B, H, N]`` (+inf where a query has no key)."""
+    if _elsewhere(qkv):
+        with torch.cuda.device(qkv.device):
+            return attention_rel_bias_train(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale)
     qkv = _bf16(qkv, "qkv")
-    with torch.cuda.device(qkv.device):
-        b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias_train")
-        out = torch.empty(b, n, num_heads * dh, dtype=qkv.dtype, device=qkv.device)
-        lse = torch.empty(b, num_heads, n, dtype=torch.float32, device=qkv.device)
-        _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(),
-                                                     lse.data_ptr(), b, num_heads, hk, dh, scale, _lib.VIT_BF16, _stream()))
+    b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias_train")
+    out = torch.empty((b, n, num_heads * dh), dtype=qkv.dtype, device=qkv.device)
+    lse = torch.empty((b, num_heads, n), dtype=torch.float32, device=qkv.device)
+    _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(),
+                                                 lse.data_ptr(), b, num_heads, hk, dh, scale, _lib.VIT_BF16, _raw_stream(qkv)))
     return out, lse
 
 
@@ -482,20 +507,24 @@ def attention_rel_bias_backward(qkv: torch.Tensor, out: torch.Tensor, d_out: tor
                                 buckets, lengths: torch.Tensor | None = None, num_kv_heads: int | None = None, scale: float | None = None):
     """Gradient of ``attention_rel_bias`` from ``attention_rel_bias_train``'s ``(out, saved)`` and the gradient of ``out``:
     ``(dqkv bf16, d_table fp32 [num_buckets, H])``. The other arguments as in the forward. Bitwise reproducible."""
+    if _elsewhere(qkv):
+        with torch.cuda.device(qkv.device):
+            return attention_rel_bias_backward(qkv, out, d_out, saved, num_heads, table, buckets, lengths, num_kv_heads, scale)
     qkv, out, d_out = _bf16(qkv, "qkv"), _bf16(out, "out"), _bf16(d_out, "d_out")
-    with torch.cuda.device(qkv.device):
-        b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias_backward")
-        for name, t, shape, dt in (("out", out, (b, n, num_heads * dh), torch.bfloat16), ("d_out", d_out, (b, n, num_heads * dh), torch.bfloat16),
-                                   ("saved", saved, (b, num_heads, n), torch.float32)):
-            if t.shape != shape or t.dtype != dt or t.device != qkv.device or not t.is_contiguous():
-                raise ValueError(f"attention_rel_bias_backward: {name} must be {dt} {shape} on {qkv.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-        lib = _lib.load()
-        c = buckets._c()
-        need = lib.vit_attention_rel_bwd_workspace_bytes(c, b, num_heads)
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=qkv.device)
-        dqkv = torch.empty_like(qkv)
-        d_table = torch.empty(buckets.num_buckets, num_heads, dtype=torch.float32, device=qkv.device)
-        _lib.check(lib.vit_attention_rel_bwd(c, qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(),
-                                             d_out.data_ptr(), saved.data_ptr(), dqkv.data_ptr(), d_table.data_ptr(), ws.data_ptr(), need,
-                                             b, num_heads, hk, dh, scale, _stream()))
+    b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias_backward")
+    wide = (b, n, num_heads * dh)
+    if out.shape != wide or d_out.shape != wide or out.device != qkv.device or d_out.device != qkv.device:
+        raise ValueError(f"attention_rel_bias_backward: out and d_out must be {wide} on {qkv.device}, got {tuple(out.shape)} on {out.device}, "
+                         f"{tuple(d_out.shape)} on {d_out.device}")
+    if saved.shape != (b, num_heads, n) or saved.dtype != torch.float32 or saved.device != qkv.device or not saved.is_contiguous():
+        raise ValueError(f"attention_rel_bias_backward: saved is not what attention_rel_bias_train returned for {tuple(qkv.shape)}")
+    lib = _lib.load()
+    c = buckets._c()
+    need = lib.vit_attention_rel_bwd_workspace_bytes(c, b, num_heads)
+    ws = torch.empty((need,), dtype=torch.uint8, device=qkv.device)
+    dqkv = torch.empty_like(qkv)
+    d_table = torch.empty((buckets.num_buckets, num_heads), dtype=torch.float32, device=qkv.device)
+    _lib.check(lib.vit_attention_rel_bwd(c, qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(), d_out.data_ptr(),
+                                         saved.data_ptr(), dqkv.data_ptr(), d_table.data_ptr(), ws.data_ptr(), need,
+                                         b, num_heads, hk, dh, scale, _raw_stream(qkv)))
     return dqkv, d_table

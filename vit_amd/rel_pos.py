@@ -93,5 +93,7 @@ class RelPosBuckets:
         return full if self.bucket_of is None else self.bucket_of.cpu().long()[full]
 
     def _c(self) -> "_lib.vit_rel_pos":
-        ptr = [None if t is None else t.data_ptr() for t in (self.bucket_of, self.by_bucket, self.bucket_start)]
-        return _lib.vit_rel_pos(self.prefix, self.grid_h, self.grid_w, self.num_buckets, *ptr)
+        if self.bucket_of is None:
+            return _lib.vit_rel_pos(self.prefix, self.grid_h, self.grid_w, self.num_buckets)
+        return _lib.vit_rel_pos(self.prefix, self.grid_h, self.grid_w, self.num_buckets, self.bucket_of.data_ptr(),
+                                self.by_bucket.data_ptr(), self.bucket_start.data_ptr())
