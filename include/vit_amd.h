@@ -286,7 +286,7 @@ int vit_attention_rel_fwd(const vit_rel_pos* pos, const void* qkv, const float* 
                           void* stream);
 /* VIT_BF16. dqkv (rows behind a sample's length: zeros) and d_table [num_buckets, heads] fp32, overwritten; d_table may be
  * NULL. No atomics: bitwise reproducible. */
-size_t vit_attention_rel_bwd_workspace_bytes(const vit_rel_pos* pos, int batch, int heads);
+size_t vit_attention_rel_bwd_workspace_bytes(const vit_rel_pos* pos, int batch, int heads, int head_dim);
 int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, const float* table, const int32_t* lengths, const void* out,
                           const void* d_out, const float* lse, void* dqkv, float* d_table, void* workspace,
                           size_t workspace_bytes, int batch, int heads, int kv_heads, int head_dim, float scale, void* stream);

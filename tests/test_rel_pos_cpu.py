@@ -147,5 +147,5 @@ def test_attention_rel_c_more_refusals():
     assert lib.vit_attention_rel_fwd(None, FAKE, FAKE, None, FAKE, None, 1, 2, 2, 32, 0.2, 1, None) == -1
     m = rel_pos(bucket_of=FAKE, num_buckets=3)  # the gradient of a mapped table without the map's inverse
     assert lib.vit_attention_rel_bwd(m, FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, 1, 2, 2, 32, 0.2, None) == -1
-    assert lib.vit_attention_rel_bwd_workspace_bytes(None, 1, 1) == 0
+    assert lib.vit_attention_rel_bwd_workspace_bytes(None, 1, 1, 32) == 0
     assert ctypes.sizeof(_lib.vit_rel_pos) == 40 and ctypes.sizeof(_lib.vit_qk_norm_config) == 48

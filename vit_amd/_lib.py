@@ -110,7 +110,7 @@ SIGNATURES = {
     "vit_qk_norm_rope_bwd_workspace_bytes": (c_size_t, [POINTER(vit_qk_norm_config)]),
     "vit_qk_norm_rope_bwd": (c_int, [POINTER(vit_qk_norm_config)] + [c_void_p] * 12 + [c_size_t, c_void_p]),
     "vit_attention_rel_fwd": (c_int, [POINTER(vit_rel_pos)] + [c_void_p] * 5 + [c_int, c_int, c_int, c_int, c_float, c_int, c_void_p]),
-    "vit_attention_rel_bwd_workspace_bytes": (c_size_t, [POINTER(vit_rel_pos), c_int, c_int]),
+    "vit_attention_rel_bwd_workspace_bytes": (c_size_t, [POINTER(vit_rel_pos), c_int, c_int, c_int]),
     "vit_attention_rel_bwd": (c_int, [POINTER(vit_rel_pos)] + [c_void_p] * 9 + [c_size_t, c_int, c_int, c_int, c_int, c_float,
                                                                              c_void_p]),
     "vit_head_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,

@@ -9,15 +9,14 @@
 //     fp32 sums of dS that make d_table. Rows of the true dS sum to zero (the P of a row sum to 1), so the row sums of the dS
 //     computed with the rounded delta, kept in fp32 beside the products, are its error: delta + sum is written for 2 and 3.
 //   2 dK, dV: 32 keys a wave on the lane, the queries of every head of the group streamed through LDS.
-//   3 bias: one 64 x 64 tile of (query, key) of one head and a range of samples per workgroup. The bias depends on the tile
-//     and not on the sample, and so does the place of dS in its gradient: dS is summed over the samples in registers, and only
-//     the sum is folded by offset (below) -- no scatter in the loop over samples. P and dP are computed again for it
-//     (2 products more), with operands straight from L2 in the MFMA's own layout.
-//   4 offsets: adds the tiles' folded sums per offset in a fixed order; 5 (only with a map) adds the offsets of a bucket.
+//   3 bias: one block of (query, key) of one head and a range of samples per workgroup. The bias depends on the pair and not on the
+//     sample, and so does the place of dS in its gradient: dS is summed over the samples in registers, and only the sum is folded by
+//     offset (below) -- no scatter in the loop over samples. P and dP are computed again for it (2 products more).
+//   4 offsets: adds the blocks' folded sums per offset in a fixed order; 5 (only with a map) adds the offsets of a bucket.
 //
-// Folding: in a tile, pair (i, j) has linear offset o = i - j in (-64, 64) + tile offset, and the grid offset is
-// dx = o mod gw (class 0: x_i >= dx, no row border between) or that - gw (class 1): 127 diagonals x 2 classes a tile, whatever
-// the grid's width, then three sums for the prefix classes.
+// Folding: pair (i, j) of a block has linear offset o = i - j, and the grid offset is dx = o mod gw (class 0: x_i >= dx, no row border
+// between) or that - gw (class 1): 2 sums for each diagonal of the block, whatever the grid's width, then three for the prefix classes.
+#include "lds_image.h"
 #include "rel_bias.h"
 #include <math.h>
 
@@ -25,9 +24,6 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 enum { MODE_DQ = 0, MODE_DKV = 1 };
-constexpr int TB = 64;              // bias tile
-constexpr int FOLD = 2 * 127 + 3;   // sums a tile leaves
-constexpr int FP = 260;             // their pitch, floats
 
 struct RelBwdArgs {
     const bf16_t* qkv;
@@ -36,14 +32,15 @@ struct RelBwdArgs {
     const float* lse;
     float* delta;  // [B, H, N]
     bf16_t* dqkv;
-    float* part;   // [splits][H][tiles][tiles][FP]
+    float* part;   // [splits][H][tq][tk][fp]: folded sums of the blocks
     float* doff;   // [H][offsets + 3] (with a map)
     float* dtable;
     const int* by_bucket;
     const int* bucket_start;
     const int* lengths;
     RelGeo geo;
-    int B, N, H, HK, IC, splits, tiles;
+    int B, N, H, HK, IC;
+    int splits, tq, tk, bq, bk, fp;  // bias gradient: sample ranges, query / key blocks, their sizes, pitch of their sums
     float scale, scale_log2e;
 };
 
@@ -259,120 +256,195 @@ __global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
     }
 }
 
-// ---- sums of dS over samples, folded by offset. Grid: (tiles * tiles, H, splits); 4 waves, a 32 x 32 quarter each
-template <int DH>
-__global__ __launch_bounds__(256) void attn_rel_bias_grad_kernel(const RelBwdArgs a) {
-    using G = BGeo<DH>;
-    __shared__ float sum[TB][TB + 1];
-    __shared__ float half[2][FOLD];
-    __shared__ float three[4][3];
+// ---- sums of dS over samples, folded by offset. Grid: (query blocks * key blocks, H, splits). A wave has 32 queries and KT tiles of
+// 32 keys; K and V of the block's keys come by LDS-DMA one sample ahead (two buffers), the wave's own Q and dO rows one sample ahead
+// in registers, so a sample costs one barrier and its loads have a sample's products to land.
+template <int DH, int KT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void attn_rel_bias_grad_kernel(const RelBwdArgs a) {
+    using I = LdsImage<DH>;
+    constexpr int KS = DH / 16, ROWS = KT * 32, IMG = ROWS * I::ROW;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    // [2][K image, V image], the keys' codes, the expansion; after the samples: [waves * 32][33] sums, then the folded vector
+    int* const codes = (int*)(smem + 4 * IMG);
+    float* const T = (float*)(codes + ROWS);
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
     const int r = lane & 31, hi = lane >> 5;
-    const int N = a.N, H = a.H, HK = a.HK;
-    const int tq = blockIdx.x / a.tiles, tk = blockIdx.x - tq * a.tiles;
+    const int N = a.N, H = a.H, HK = a.HK, B = a.B;
+    const int tq = blockIdx.x / a.tk, tk = blockIdx.x - tq * a.tk;
     const int h = blockIdx.y, hk = h / (H / HK);
-    const int iq = (wave >> 1) * 32, ik = (wave & 1) * 32;  // this wave's quarter
-    const int q0 = tq * TB + iq, k0 = tk * TB + ik;
-    const int q = q0 + r;
-    const size_t rs = (size_t)(H + 2 * HK) * DH, os = (size_t)H * DH;
-    const int b0 = (int)((int64_t)a.B * blockIdx.z / a.splits), b1 = (int)((int64_t)a.B * (blockIdx.z + 1) / a.splits);
-
-    // bias of the quarter (register e: key, lane: query)
-    f32x16 bias, acc;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int k = k0 + (e & 3) + 8 * (e >> 2) + 4 * hi;
-        const bool qp = q < a.geo.prefix, kp = k < a.geo.prefix;
-        const int at = qp ? (kp ? a.geo.offsets + 2 : a.geo.offsets)
-                          : kp ? a.geo.offsets + 1 : rel_code(a.geo, q < N ? q : N - 1) - rel_code(a.geo, k < N ? k : N - 1) + a.geo.center;
-        bias[e] = rel_entry(a.geo, at, h);
-        acc[e] = 0.f;
-    }
-    if (q0 < N && k0 < N) {
-        for (int b = b0; b < b1; ++b) {
-            const int nb = sample_length(a.lengths, b, N);
-            if (q0 >= nb || k0 >= nb) continue;
-            const int qr = q < nb ? q : nb - 1, kr = k0 + r < nb ? k0 + r : nb - 1;
-            const bf16_t* base = a.qkv + (size_t)b * N * rs;
-            const bf16_t* qp = base + (size_t)qr * rs + (size_t)h * DH + hi * 8;
-            const bf16_t* dp_ = a.dout + ((size_t)b * N + qr) * os + (size_t)h * DH + hi * 8;
-            const bf16_t* kp = base + (size_t)kr * rs + (size_t)(H + hk) * DH + hi * 8;
-            const bf16_t* vp = kp + (size_t)HK * DH;
-            const size_t sat = ((size_t)b * H + h) * N;
-            const float L = q < nb ? a.lse[sat + q] : INFINITY;
-            const float D = a.delta[sat + qr];
-            f32x16 s = bias, dp;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dp[e] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < G::KSTEPS; ++ks) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kp + ks * 16), *(const bf16x8*)(qp + ks * 16), s, 0, 0, 0);
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(vp + ks * 16), *(const bf16x8*)(dp_ + ks * 16), dp, 0, 0, 0);
-            }
-            if (k0 + 32 > nb) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (k0 + (e & 3) + 8 * (e >> 2) + 4 * hi >= nb) s[e] = -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L);
-                acc[e] += p * (dp[e] - D);
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sum[iq + r][ik + (e & 3) + 8 * (e >> 2) + 4 * hi] = acc[e];
+    const int blk0 = tq * nw * 32, q0 = blk0 + wave * 32, q = q0 + r, k0 = tk * ROWS;
+    const int pitch = (H + 2 * HK) * DH * 2, opitch = H * DH * 2;
+    const int b0 = (int)((int64_t)B * blockIdx.z / a.splits), b1 = (int)((int64_t)B * (blockIdx.z + 1) / a.splits);
+    const int blk1 = blk0 + nw * 32 < N ? blk0 + nw * 32 - 1 : N - 1;
+    const RelSlice sl(a.geo, blk0, blk1, true);
+    rel_expand(a.geo, T, sl.lo, sl.n, h);
+    for (int i = tid; i < ROWS; i += blockDim.x) codes[i] = rel_code(a.geo, k0 + i);
+    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - sl.lo;
     __syncthreads();
 
-    // fold: thread = (diagonal, half of the rows)
+    auto next_sample = [&](int b) {  // the first from b on that has a pair in this block
+        while (b < b1) {
+            const int nb = sample_length(a.lengths, b, N);
+            if (nb > blk0 && nb > k0) break;
+            ++b;
+        }
+        return b;
+    };
+    auto stage = [&](int b, int buf) {
+        const int nb = sample_length(a.lengths, b, N);
+        const char* base = (const char*)a.qkv + (size_t)b * N * pitch + (size_t)(H + hk) * DH * 2;
+        const __amdgpu_buffer_rsrc_t kr = head_resource<DH>(base, N, pitch), vr = head_resource<DH>(base + (size_t)HK * DH * 2, N, pitch);
+        unsigned char* const dst = smem + buf * 2 * IMG;
+        // whole tiles up to the sample's last key (rows behind it re-read that key: what is masked is still finite)
+        const int need = nb - k0 < ROWS ? (nb - k0 + 31) & ~31 : ROWS;
+        for (int i = wave * I::RPI; i < need; i += nw * I::RPI) {
+            I::dma(kr, dst, i, ROWS, k0, nb - 1, pitch, lane);
+            I::dma(vr, dst + IMG, i, ROWS, k0, nb - 1, pitch, lane);
+        }
+    };
+    bf16x8 fq[KS], fo[KS], nq[KS], no[KS];
+    float L = INFINITY, D = 0.f, nL = INFINITY, nD = 0.f;
+    auto load_rows = [&](int b) {
+        const int nb = sample_length(a.lengths, b, N);
+        const int qr = q < nb ? q : nb - 1;
+        const char* qp = (const char*)a.qkv + (size_t)b * N * pitch + (size_t)qr * pitch + (size_t)h * DH * 2 + hi * 16;
+        const char* op = (const char*)a.dout + ((size_t)b * N + qr) * opitch + (size_t)h * DH * 2 + hi * 16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            nq[ks] = *(const bf16x8*)(qp + ks * 32);
+            no[ks] = *(const bf16x8*)(op + ks * 32);
+        }
+        const size_t at = ((size_t)b * H + h) * N + qr;
+        nL = q < nb ? a.lse[at] : INFINITY;  // P = exp2(.. - inf) = 0 for rows behind the sample
+        nD = a.delta[at];
+    };
+    f32x16 acc[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+
+    int b = next_sample(b0), buf = 0;
+    if (b < b1) {
+        load_rows(b);
+        stage(b, 0);
+    }
+    while (b < b1) {
+        const int nb = sample_length(a.lengths, b, N), bn = next_sample(b + 1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // this sample's images are whole; nobody reads the other buffer any more
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) { fq[ks] = nq[ks]; fo[ks] = no[ks]; }
+        L = nL;
+        D = nD;
+        if (bn < b1) {
+            load_rows(bn);
+            stage(bn, buf ^ 1);
+        }
+        const unsigned char* Kb = smem + buf * 2 * IMG;
+        if (q0 < nb) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const int key0 = k0 + t * 32;
+                if (key0 < nb) {
+                    f32x16 s, dp;
+                    rel_tile<true>(s, T, codes + t * 32, qcode, hi, a.geo.prefix, sl.n, q, key0);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const int off = I::at(t * 32 + r, ks * 2 + hi);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + off), fq[ks], s, 0, 0, 0);
+                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + IMG + off), fo[ks], dp, 0, 0, 0);
+                    }
+                    if (key0 + 32 > nb) {
+                        int lim = nb - key0 - 4 * hi;
+                        asm volatile("" : "+v"(lim));
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L);
+                        acc[t][e] = fmaf(p, dp[e] - D, acc[t][e]);
+                    }
+                }
+            }
+        }
+        b = bn;
+        buf ^= 1;
+    }
+
+    // ---- fold, one strip of 32 keys at a time: thread = diagonal i - j of the strip; vector place v = its offset from the block's lowest
+    const int nq32 = nw * 32, nd = nq32 + 31;
+    float* const S = (float*)smem;         // [nq32][33]
+    float* const V = S + nq32 * 33;        // [2 (nq32 + ROWS - 1)]
+    float* const P3 = V + 2 * (nq32 + ROWS - 1);  // [8][3]
     const int prefix = a.geo.prefix, gw = a.geo.gw;
-    const int tq0 = tq * TB, tk0 = tk * TB;
-    {
-        const int dg = tid & 127, part = tid >> 7;  // diagonal dg: i - j = dg - 63 inside the tile
-        if (dg < 127) {
-            const int o = tq0 - tk0 + dg - 63;  // query token - key token
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f;
+    __syncthreads();
+    for (int i = tid; i < 2 * (nq32 + ROWS - 1); i += blockDim.x) V[i] = 0.f;
+    for (int t = 0; t < KT && k0 + t * 32 < N; ++t) {
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+            if (u != t) continue;  // (uniform; the accumulators need constant indices)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) S[(wave * 32 + r) * 33 + (e & 3) + 8 * (e >> 2) + 4 * hi] = acc[u][e];
+        }
+        __syncthreads();
+        for (int g = tid; g < nd; g += blockDim.x) {
+            const int o = blk0 - (k0 + t * 32) + g - 31;  // query token - key token
             int dx = o % gw;
             if (dx < 0) dx += gw;
-            float s0 = 0.f, s1 = 0.f;
-            for (int i = part * 32; i < part * 32 + 32; ++i) {
-                const int j = i - (dg - 63);
-                if (j < 0 || j >= TB) continue;
-                const int p = tq0 + i - prefix;
-                if (p < 0 || tk0 + j < prefix || tq0 + i >= N || tk0 + j >= N) continue;
-                const float v = sum[i][j];
-                if (p % gw >= dx) s0 += v; else s1 += v;
+            int p = blk0 + g - 31 - prefix;  // place of the query at j = 0
+            int x = p % gw;
+            if (x < 0) x += gw;
+            float a0 = 0.f, a1 = 0.f;
+            for (int j = 0; j < 32; ++j) {
+                const int i = g - 31 + j, key = k0 + t * 32 + j;
+                if (i >= 0 && i < nq32 && p + j >= 0 && key >= prefix && blk0 + i < N && key < N) {
+                    const float v = S[i * 33 + j];
+                    if (x >= dx) a0 += v; else a1 += v;
+                }
+                x = x + 1 == gw ? 0 : x + 1;
             }
-            half[part][2 * dg] = s0;
-            half[part][2 * dg + 1] = s1;
+            const int v = g + 32 * (KT - 1 - t);
+            V[2 * v] += a0;
+            V[2 * v + 1] += a1;
+        }
+        if (prefix > 0 && (tq == 0 || tk == 0) && tid < nq32) {
+            const int tokq = blk0 + tid;
+            for (int j = 0; j < 32; ++j) {
+                const int key = k0 + t * 32 + j;
+                if (tokq >= N || key >= N) continue;
+                const float v = S[tid * 33 + j];
+                if (tokq < prefix) {
+                    if (key < prefix) s2 += v; else s0 += v;
+                } else if (key < prefix) {
+                    s1 += v;
+                }
+            }
         }
     }
-    if (prefix > 0 && (tq == 0 || tk == 0)) {  // prefix pairs of this tile: 16 columns of a row a thread
-        const int i = tid >> 2, jb = (tid & 3) * 16;
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f;
-        for (int j = jb; j < jb + 16; ++j) {
-            if (tq0 + i >= N || tk0 + j >= N) continue;
-            const bool qp = tq0 + i < prefix, kp = tk0 + j < prefix;
-            const float v = sum[i][j];
-            if (qp && !kp) s0 += v;
-            if (!qp && kp) s1 += v;
-            if (qp && kp) s2 += v;
-        }
-        s0 = wave_sum(s0);
-        s1 = wave_sum(s1);
-        s2 = wave_sum(s2);
-        if (lane == 0) { three[wave][0] = s0; three[wave][1] = s1; three[wave][2] = s2; }
-    } else if (lane == 0) {
-        three[wave][0] = three[wave][1] = three[wave][2] = 0.f;
-    }
+    s0 = wave_sum(s0);
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if (lane == 0) { P3[wave * 3] = s0; P3[wave * 3 + 1] = s1; P3[wave * 3 + 2] = s2; }
     __syncthreads();
-    float* dst = a.part + ((((size_t)blockIdx.z * H + h) * a.tiles + tq) * a.tiles + tk) * FP;
-    for (int i = tid; i < FOLD; i += 256)
-        dst[i] = i < 254 ? half[0][i] + half[1][i] : (three[0][i - 254] + three[1][i - 254]) + (three[2][i - 254] + three[3][i - 254]);
+    const int fold = 2 * (nq32 + ROWS - 1);
+    float* dst = a.part + ((((size_t)blockIdx.z * H + h) * a.tq + tq) * a.tk + tk) * a.fp;
+    for (int i = tid; i < fold; i += blockDim.x) dst[i] = V[i];
+    if (tid < 3) {
+        float v = 0.f;
+        for (int w = 0; w < nw; ++w) v += P3[w * 3 + tid];
+        dst[fold + tid] = v;
+    }
 }
 
-// ---- per offset: the tiles' folded sums in a fixed order. One wave per (offset index, head): lanes over (split, query tile)
+// ---- per offset: the blocks' folded sums in a fixed order. One wave per (offset index, head): lanes over (split, query block)
 __global__ __launch_bounds__(256) void attn_rel_offset_kernel(const RelBwdArgs a, float* dst, int stride_h, int stride_o) {
     const int lane = threadIdx.x & 63;
     const int idx = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
@@ -381,23 +453,19 @@ __global__ __launch_bounds__(256) void attn_rel_offset_kernel(const RelBwdArgs a
     const int gw = a.geo.gw, rows = 2 * gw - 1;
     const int dyi = idx / rows, dx = idx - dyi * rows - (gw - 1), dy = dyi - (a.geo.center / rows);
     const int o = dy * gw + dx, cls = dx < 0 ? 1 : 0;
+    const int bq = a.bq, bk = a.bk, fold = bq + bk - 1;  // queries, keys of a block, diagonals
     float s = 0.f;
-    for (int i = lane; i < a.splits * a.tiles; i += 64) {
-        const int sp = i / a.tiles, tq = i - sp * a.tiles;
-        const float* p = a.part + (((size_t)sp * a.H + h) * a.tiles + tq) * a.tiles * FP;
+    for (int i = lane; i < a.splits * a.tq; i += 64) {
+        const int sp = i / a.tq, tq = i - sp * a.tq;
+        const float* p = a.part + (((size_t)sp * a.H + h) * a.tq + tq) * a.tk * a.fp;
         if (idx >= offsets) {
-            for (int tk = 0; tk < a.tiles; ++tk)
-                if (tq == 0 || tk == 0) s += p[(size_t)tk * FP + 254 + idx - offsets];
+            for (int tk = 0; tk < a.tk; ++tk)
+                if (tq == 0 || tk == 0) s += p[(size_t)tk * a.fp + 2 * fold + idx - offsets];
         } else {
-            // keys j = i - o of the tile's 64 queries: at most two key tiles
-            const int j0 = tq * TB - o;                      // key of the tile's first query
-            const int t0 = j0 >= 0 ? j0 / TB : -((-j0 + TB - 1) / TB);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int tk = t0 + k;
-                const int dg = o - (tq - tk) * TB + 63;
-                if (tk >= 0 && tk < a.tiles && dg >= 0 && dg < 127) s += p[(size_t)tk * FP + 2 * dg + cls];
-            }
+            // key blocks that hold a key i - o of the block's queries
+            const int j0 = tq * bq - o, j1 = j0 + bq - 1;  // keys of its first and last query
+            const int t0 = j0 > 0 ? j0 / bk : 0, t1 = j1 < 0 ? -1 : j1 / bk;
+            for (int tk = t0; tk <= t1 && tk < a.tk; ++tk) s += p[(size_t)tk * a.fp + 2 * (o - (tq * bq - tk * bk) + bk - 1) + cls];
         }
     }
     s = wave_sum(s);
@@ -463,28 +531,57 @@ int launch_part(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
     return VIT_OK;
 }
 
-// how many workgroups share a bias tile's samples: enough of them to fill the chip, whole samples each
-int bias_splits(int batch, int heads, int tiles, int ncu) {
-    const int64_t have = (int64_t)heads * tiles * tiles;
-    int64_t s = (4LL * ncu + have - 1) / have;
-    if (s > batch) s = batch;
-    return s < 1 ? 1 : (int)s;
-}
 struct Workspace {
     size_t delta, part, doff, bytes;
-    int tiles, splits;
+    int splits, tq, tk, bq, bk, fp;
 };
-int plan_workspace(const vit_rel_pos* pos, int batch, int heads, Workspace* w) {
+// LDS of the bias gradient's workgroups: two buffers of K and V images, codes, expansion
+size_t bias_lds(int head_dim, int kt, int slice) {
+    const int ch = head_dim / 8, row = (ch == 8 || ch == 16 ? ch : ch + 1) * 16;
+    return (size_t)4 * kt * 32 * row + (size_t)(kt * 32 + slice) * 4;
+}
+int plan_workspace(const vit_rel_pos* pos, int batch, int heads, int head_dim, Workspace* w) {
     int ncu = 0;
     VIT_TRY_RC(vit_cu_count(&ncu));
-    const int N = pos->prefix + pos->grid_h * pos->grid_w;
-    w->tiles = ceil_div(N, TB);
-    w->splits = bias_splits(batch, heads, w->tiles, ncu);
+    const int N = pos->prefix + pos->grid_h * pos->grid_w, n32 = ceil_div(N, 32);
+    // query blocks of up to 8 waves, all alike; key blocks of 7 tiles where that is the whole sequence (one block: Q, dO, K, V are read
+    // once a sample) and the head dim leaves the registers room for it, else 4 tiles, 2 where the expansion of a long sequence
+    // leaves the images less
+    w->tq = ceil_div(n32, 8);
+    w->bq = ceil_div(n32, w->tq) * 32;
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, w->bq);
+    w->bk = (head_dim <= 64 && n32 > 4 && n32 <= 7 ? 7 : bias_lds(head_dim, 4, slice) <= 160 * 1024 ? 4 : 2) * 32;
+    w->tk = ceil_div(N, w->bk);
+    w->fp = 2 * (w->bq + w->bk - 1) + 4;
+    // enough sample ranges to give every CU a workgroup, whole samples each
+    int64_t s = ncu / ((int64_t)heads * w->tq * w->tk);
+    w->splits = s < 1 ? 1 : s > batch ? batch : (int)s;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     w->delta = 0;
     w->part = up((size_t)batch * heads * N * 4);
-    w->doff = w->part + up((size_t)w->splits * heads * w->tiles * w->tiles * FP * 4);
+    w->doff = w->part + up((size_t)w->splits * heads * w->tq * w->tk * w->fp * 4);
     w->bytes = w->doff + up((size_t)heads * ((size_t)(2 * pos->grid_h - 1) * (2 * pos->grid_w - 1) + 3) * 4);
+    return VIT_OK;
+}
+
+template <int DH, int KT>
+int launch_bias_grad(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t stream) {
+    const int nw = a.bq / 32;
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, a.bq);
+    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
+    size_t lds = bias_lds(DH, KT, slice);
+    const size_t fold = ((size_t)a.bq * 33 + 2 * (a.bq + KT * 32 - 1) + 24) * 4;
+    if (lds < fold) lds = fold;
+    VIT_REQUIRE(lds <= 160 * 1024, "attention_rel_bwd: head_dim %d with %d bias entries does not fit the LDS", DH, slice);
+    auto kern = attn_rel_bias_grad_kernel<DH, KT>;
+    static PerDeviceInt attr_set;
+    std::atomic<int>* as = attr_set.slot();
+    if (!as || !as->load(std::memory_order_relaxed)) {
+        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (as) as->store(1, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(kern, dim3(a.tq * a.tk, a.H, a.splits), dim3(nw * 64), lds, stream, a);
+    VIT_CHECK_HIP(hipGetLastError());
     return VIT_OK;
 }
 
@@ -493,8 +590,9 @@ int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
     VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, stream)));
     VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, stream)));
     if (!a.dtable) return VIT_OK;
-    hipLaunchKernelGGL(attn_rel_bias_grad_kernel<DH>, dim3(a.tiles * a.tiles, a.H, a.splits), dim3(256), 0, stream, a);
-    VIT_CHECK_HIP(hipGetLastError());
+    if (a.bk == 7 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 64 ? 7 : 4)>(a, pos, stream)));
+    else if (a.bk == 4 * 32) VIT_TRY_RC((launch_bias_grad<DH, 4>(a, pos, stream)));
+    else VIT_TRY_RC((launch_bias_grad<DH, 2>(a, pos, stream)));
     const int total = a.geo.offsets + (a.geo.prefix ? 3 : 0);
     // without a map, and with nothing in the table behind the offsets, the offset sums are the table's gradient
     const bool direct = !a.geo.bucket_of && a.geo.num_buckets == total;
@@ -510,10 +608,10 @@ int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
 
 }  // namespace
 
-extern "C" size_t vit_attention_rel_bwd_workspace_bytes(const vit_rel_pos* pos, int batch, int heads) {
+extern "C" size_t vit_attention_rel_bwd_workspace_bytes(const vit_rel_pos* pos, int batch, int heads, int head_dim) {
     Workspace w{};
     if (!pos || batch <= 0 || heads <= 0 || pos->prefix < 0 || pos->grid_h <= 0 || pos->grid_w <= 0 ||
-        (int64_t)pos->grid_h * pos->grid_w > 16384 || plan_workspace(pos, batch, heads, &w) != VIT_OK)
+        (int64_t)pos->grid_h * pos->grid_w > 16384 || plan_workspace(pos, batch, heads, head_dim, &w) != VIT_OK)
         return 0;
     return w.bytes;
 }
@@ -531,10 +629,11 @@ extern "C" int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, co
                 "vit_attention_rel_bwd: tensors must be 16-byte aligned");
     RelBwdArgs a{};
     VIT_TRY_RC(rel_make_geo("vit_attention_rel_bwd", pos, table, heads, scale, &a.geo, &a.N));
+    VIT_REQUIRE((int64_t)a.N * (heads + 2 * kv_heads) * head_dim * 2 < (1LL << 31), "vit_attention_rel_bwd: one sample's qkv rows exceed 2 GiB");
     VIT_REQUIRE(!d_table || !pos->bucket_of || (pos->by_bucket && pos->bucket_start),
                 "vit_attention_rel_bwd: the gradient of a mapped table needs the map's inverse");
     Workspace w{};
-    VIT_TRY_RC(plan_workspace(pos, batch, heads, &w));
+    VIT_TRY_RC(plan_workspace(pos, batch, heads, head_dim, &w));
     if (workspace_bytes < w.bytes)
         return vit_set_error(VIT_E_NOMEM, "vit_attention_rel_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, w.bytes);
     a.qkv = (const bf16_t*)qkv;
@@ -553,7 +652,11 @@ extern "C" int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, co
     a.H = heads;
     a.HK = kv_heads;
     a.splits = w.splits;
-    a.tiles = w.tiles;
+    a.tq = w.tq;
+    a.tk = w.tk;
+    a.bq = w.bq;
+    a.bk = w.bk;
+    a.fp = w.fp;
     a.scale = scale;
     a.scale_log2e = scale * LOG2E;
 #define RELB_CASE(DHV) \

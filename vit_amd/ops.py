@@ -520,7 +520,7 @@ def attention_rel_bias_backward(qkv: torch.Tensor, out: torch.Tensor, d_out: tor
         raise ValueError(f"attention_rel_bias_backward: saved is not what attention_rel_bias_train returned for {tuple(qkv.shape)}")
     lib = _lib.load()
     c = buckets._c()
-    need = lib.vit_attention_rel_bwd_workspace_bytes(c, b, num_heads)
+    need = lib.vit_attention_rel_bwd_workspace_bytes(c, b, num_heads, dh)
     ws = torch.empty((need,), dtype=torch.uint8, device=qkv.device)
     dqkv = torch.empty_like(qkv)
     d_table = torch.empty((buckets.num_buckets, num_heads), dtype=torch.float32, device=qkv.device)
