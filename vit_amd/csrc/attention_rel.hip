@@ -72,8 +72,8 @@ __global__ __launch_bounds__(512) void attention_rel_bf16_kernel(const RelFwdArg
 
     const int blk1 = blk0 + nwaves * 32 - 1;
     const RelSlice sl(a.geo, blk0, blk1 < N ? blk1 : N - 1, true);
-    rel_expand(a.geo, T, sl.lo, sl.n, h);
-    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - sl.lo;
+    rel_expand(a.geo, T, sl, true, h);
+    const RelLane<true> rl(a.geo, sl, T, q, N - 1);
 
     f32x16 o[G::DB];
 #pragma unroll
@@ -98,13 +98,13 @@ __global__ __launch_bounds__(512) void attention_rel_bf16_kernel(const RelFwdArg
             *(bf16x8*)(Kl + (size_t)key * G::KS + c * 16) = *(const bf16x8*)(kbase + (size_t)gk * rs + c * 8);
             *(bf16x8*)(Vl + (size_t)key * G::VS + c * 16) = *(const bf16x8*)(vbase + (size_t)gk * rs + c * 8);
         }
-        for (int i = tid; i < nkeys; i += blockDim.x) codes[i] = rel_code(a.geo, kc0 + i);
+        for (int i = tid; i < nkeys; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, kc0 + i);
         __syncthreads();
 
         for (int t = 0; t < nkeys >> 5; ++t) {
             const int key0 = kc0 + t * 32;
             f32x16 s;
-            rel_tile<true>(s, T, codes + t * 32, qcode, hi, a.geo.prefix, sl.n, q, key0);
+            rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
             const unsigned char* kp = Kl + (size_t)(t * 32 + r) * G::KS + hi * 16;
 #pragma unroll
             for (int ks = 0; ks < G::KSTEPS; ++ks)
@@ -205,8 +205,8 @@ __global__ __launch_bounds__(512) void attention_rel_f32_kernel(const RelFwdArgs
 
     const int blk1 = blk0 + nwaves * 32 - 1;
     const RelSlice sl(a.geo, blk0, blk1 < N ? blk1 : N - 1, true);
-    rel_expand(a.geo, T, sl.lo, sl.n, h);
-    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - sl.lo;
+    rel_expand(a.geo, T, sl, true, h);
+    const RelLane<true> rl(a.geo, sl, T, q, N - 1);
 
     f32x16 o[DB];
 #pragma unroll
@@ -230,13 +230,13 @@ __global__ __launch_bounds__(512) void attention_rel_f32_kernel(const RelFwdArgs
             if (c < DH) Kl[(size_t)key * KSF + c] = kv;
             Vl[(size_t)key * VSF + c] = vv;
         }
-        for (int i = tid; i < nkeys; i += blockDim.x) codes[i] = rel_code(a.geo, kc0 + i);
+        for (int i = tid; i < nkeys; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, kc0 + i);
         __syncthreads();
 
         for (int t = 0; t < nkeys >> 5; ++t) {
             const int key0 = kc0 + t * 32;
             f32x16 s;
-            rel_tile<true>(s, T, codes + t * 32, qcode, hi, a.geo.prefix, sl.n, q, key0);
+            rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
             const float* kp = Kl + (size_t)(t * 32 + r) * KSF + hi;
 #pragma unroll
             for (int kk = 0; kk < DH / 2; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kp[2 * kk], qf[kk], s, 0, 0, 0);

@@ -20,6 +20,11 @@
 #include "rel_bias.h"
 #include <math.h>
 
+// launches 1 and 2 in one pass where a head fits the LDS (attention_rel_bwd_dh64.hip)
+bool attention_rel_bwd_dh64_eligible(int N, int heads, int kv_heads, int head_dim);
+int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,
+                                  const int* lengths, int batch, int N, int heads, float scale, hipStream_t stream);
+
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -137,15 +142,13 @@ __global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
         for (int e = 0; e < 16; ++e) { acc1[d][e] = 0.f; acc2[d][e] = 0.f; }
 
     const RelSlice sl(a.geo, blk0, blk1, MODE == MODE_DQ);  // over all keys / all queries
-    const int oc = rel_code(a.geo, row < N ? row : N - 1);
+    const RelLane<MODE == MODE_DQ> rl(a.geo, sl, T, row, N - 1);
     const int nheads = MODE == MODE_DQ ? 1 : group;
     float dsum = 0.f;  // DQ: row sum of dS
     for (int gh = 0; gh < nheads && nb > 0; ++gh) {
         const int h = MODE == MODE_DQ ? oh : oh * group + gh;
-        const int lane_code = MODE == MODE_DQ ? oc + a.geo.center - sl.lo : oc;
-        const int row_add = MODE == MODE_DQ ? 0 : a.geo.center - sl.lo;
         __syncthreads();
-        rel_expand(a.geo, T, sl.lo, sl.n, h);
+        rel_expand(a.geo, T, sl, MODE == MODE_DQ, h);
         const bf16_t* i1 = MODE == MODE_DQ ? kbase : base + (size_t)h * DH;
         const bf16_t* i2 = MODE == MODE_DQ ? vbase : a.dout + (size_t)b * N * os + (size_t)h * DH;
         const size_t s2 = MODE == MODE_DQ ? rs : os;
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
             }
             for (int i = tid; i < nin; i += blockDim.x) {
                 const int gr = ic0 + i;
-                codes[i] = rel_code(a.geo, gr) + row_add;
+                codes[i] = rel_row_code(a.geo, sl, MODE == MODE_DQ, gr);
                 if constexpr (MODE == MODE_DKV) {
                     rowL[i] = gr < nb ? a.lse[sat + gr] : INFINITY;  // P = exp2(.. - inf) = 0 for pad queries
                     rowD[i] = gr < nb ? a.delta[sat + gr] : 0.f;
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
             __syncthreads();
             for (int t = 0; t < nin >> 5; ++t) {
                 f32x16 s, dp;
-                rel_tile<MODE == MODE_DQ>(s, T, codes + t * 32, lane_code, hi, a.geo.prefix, sl.n, row, ic0 + t * 32);
+                rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, ic0 + t * 32);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dp[e] = 0.f;
                 const unsigned char* p1 = R1 + (size_t)(t * 32 + r) * G::RS + hi * 16;
@@ -278,9 +281,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
     const int b0 = (int)((int64_t)B * blockIdx.z / a.splits), b1 = (int)((int64_t)B * (blockIdx.z + 1) / a.splits);
     const int blk1 = blk0 + nw * 32 < N ? blk0 + nw * 32 - 1 : N - 1;
     const RelSlice sl(a.geo, blk0, blk1, true);
-    rel_expand(a.geo, T, sl.lo, sl.n, h);
-    for (int i = tid; i < ROWS; i += blockDim.x) codes[i] = rel_code(a.geo, k0 + i);
-    const int qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - sl.lo;
+    rel_expand(a.geo, T, sl, true, h);
+    for (int i = tid; i < ROWS; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, k0 + i);
+    const RelLane<true> rl(a.geo, sl, T, q, N - 1);
     __syncthreads();
 
     auto next_sample = [&](int b) {  // the first from b on that has a pair in this block
@@ -291,33 +294,44 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
         }
         return b;
     };
-    auto stage = [&](int b, int buf) {
-        const int nb = sample_length(a.lengths, b, N);
+    // a part of a sample's loads: this wave's pieces i0, i0 + 1 .. of the K and V images, part of its query rows
+    const int pieces = (ROWS + nw * I::RPI - 1) / (nw * I::RPI);  // a wave has per image
+    auto stage = [&](int b, int nb, int buf, int i0, int i1) {
         const char* base = (const char*)a.qkv + (size_t)b * N * pitch + (size_t)(H + hk) * DH * 2;
         const __amdgpu_buffer_rsrc_t kr = head_resource<DH>(base, N, pitch), vr = head_resource<DH>(base + (size_t)HK * DH * 2, N, pitch);
         unsigned char* const dst = smem + buf * 2 * IMG;
         // whole tiles up to the sample's last key (rows behind it re-read that key: what is masked is still finite)
         const int need = nb - k0 < ROWS ? (nb - k0 + 31) & ~31 : ROWS;
-        for (int i = wave * I::RPI; i < need; i += nw * I::RPI) {
-            I::dma(kr, dst, i, ROWS, k0, nb - 1, pitch, lane);
-            I::dma(vr, dst + IMG, i, ROWS, k0, nb - 1, pitch, lane);
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // (opaque: the lane offsets are made here, not kept in registers over the products)
+        for (int i = i0; i < i1; ++i) {
+            const int row = (i * nw + wave) * I::RPI;
+            if (row < need) {
+                I::dma(kr, dst, row, ROWS, k0, nb - 1, pitch, ln);
+                I::dma(vr, dst + IMG, row, ROWS, k0, nb - 1, pitch, ln);
+            }
         }
     };
     bf16x8 fq[KS], fo[KS], nq[KS], no[KS];
     float L = INFINITY, D = 0.f, nL = INFINITY, nD = 0.f;
-    auto load_rows = [&](int b) {
-        const int nb = sample_length(a.lengths, b, N);
-        const int qr = q < nb ? q : nb - 1;
-        const char* qp = (const char*)a.qkv + (size_t)b * N * pitch + (size_t)qr * pitch + (size_t)h * DH * 2 + hi * 16;
-        const char* op = (const char*)a.dout + ((size_t)b * N + qr) * opitch + (size_t)h * DH * 2 + hi * 16;
+    auto load_rows = [&](int b, int nb, int ks0, int ks1) {
+        int ql = q;
+        asm volatile("" : "+v"(ql));
+        const int qr = ql < nb ? ql : nb - 1;
+        const char* qp = (const char*)a.qkv + (size_t)b * N * pitch + (size_t)h * DH * 2;  // (uniform bases, 32-bit lane offsets)
+        const char* op = (const char*)a.dout + (size_t)b * N * opitch + (size_t)h * DH * 2;
+        const unsigned qo = (unsigned)(qr * pitch + hi * 16), oo = (unsigned)(qr * opitch + hi * 16);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            nq[ks] = *(const bf16x8*)(qp + ks * 32);
-            no[ks] = *(const bf16x8*)(op + ks * 32);
+            if (ks < ks0 || ks >= ks1) continue;
+            nq[ks] = *(const bf16x8*)(qp + qo + ks * 32);
+            no[ks] = *(const bf16x8*)(op + oo + ks * 32);
         }
-        const size_t at = ((size_t)b * H + h) * N + qr;
-        nL = q < nb ? a.lse[at] : INFINITY;  // P = exp2(.. - inf) = 0 for rows behind the sample
-        nD = a.delta[at];
+        if (ks1 == KS) {
+            const size_t at = ((size_t)b * H + h) * N;
+            nL = (a.lse + at)[qr];
+            nD = (a.delta + at)[qr];
+        }
     };
     f32x16 acc[KT];
 #pragma unroll
@@ -326,54 +340,51 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
         for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
 
     int b = next_sample(b0), buf = 0;
+    int nb = b < b1 ? sample_length(a.lengths, b, N) : 0;
     if (b < b1) {
-        load_rows(b);
-        stage(b, 0);
+        load_rows(b, nb, 0, KS);
+        stage(b, nb, 0, 0, pieces);
     }
     while (b < b1) {
-        const int nb = sample_length(a.lengths, b, N), bn = next_sample(b + 1);
+        const int bn = next_sample(b + 1), nnb = bn < b1 ? sample_length(a.lengths, bn, N) : 0;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // this sample's images are whole; nobody reads the other buffer any more
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) { fq[ks] = nq[ks]; fo[ks] = no[ks]; }
-        L = nL;
+        L = q < nb ? nL : INFINITY;  // P = exp2(.. - inf) = 0 for rows behind the sample
         D = nD;
-        if (bn < b1) {
-            load_rows(bn);
-            stage(bn, buf ^ 1);
-        }
         const unsigned char* Kb = smem + buf * 2 * IMG;
-        if (q0 < nb) {
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const int key0 = k0 + t * 32;
-                if (key0 < nb) {
-                    f32x16 s, dp;
-                    rel_tile<true>(s, T, codes + t * 32, qcode, hi, a.geo.prefix, sl.n, q, key0);
+        for (int t = 0; t < KT; ++t) {
+            const int key0 = k0 + t * 32;
+            if (bn < b1) {  // the next sample's loads, some a tile: all at once they would block the wave at the CU's memory queue
+                load_rows(bn, nnb, t * KS / KT, (t + 1) * KS / KT);
+                stage(bn, nnb, buf ^ 1, t * pieces / KT, (t + 1) * pieces / KT);
+            }
+            if (q0 < nb && key0 < nb) {
+                f32x16 s, dp;
+                rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+                for (int e = 0; e < 16; ++e) dp[e] = -D;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const int off = I::at(t * 32 + r, ks * 2 + hi);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + off), fq[ks], s, 0, 0, 0);
-                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + IMG + off), fo[ks], dp, 0, 0, 0);
-                    }
-                    if (key0 + 32 > nb) {
-                        int lim = nb - key0 - 4 * hi;
-                        asm volatile("" : "+v"(lim));
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L);
-                        acc[t][e] = fmaf(p, dp[e] - D, acc[t][e]);
-                    }
+                for (int ks = 0; ks < KS; ++ks) {
+                    const int off = I::at(t * 32 + r, ks * 2 + hi);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + off), fq[ks], s, 0, 0, 0);
+                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + IMG + off), fo[ks], dp, 0, 0, 0);
                 }
+                if (key0 + 32 > nb) {
+                    int lim = nb - key0 - 4 * hi;
+                    asm volatile("" : "+v"(lim));
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(__builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L), dp[e], acc[t][e]);
             }
         }
         b = bn;
+        nb = nnb;
         buf ^= 1;
     }
 
@@ -399,16 +410,21 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
             const int o = blk0 - (k0 + t * 32) + g - 31;  // query token - key token
             int dx = o % gw;
             if (dx < 0) dx += gw;
-            int p = blk0 + g - 31 - prefix;  // place of the query at j = 0
+            const int p = blk0 + g - 31 - prefix;  // place of the query at j = 0
             int x = p % gw;
             if (x < 0) x += gw;
+            // the diagonal's pairs: rows 0 .. nq32 - 1 of the strip, both tokens on the grid and in the sequence
+            int j0 = 31 - g > -p ? 31 - g : -p, j1 = nq32 + 31 - g;
+            if (prefix - (k0 + t * 32) > j0) j0 = prefix - (k0 + t * 32);
+            if (N - (k0 + t * 32) < j1) j1 = N - (k0 + t * 32);
+            if (N - (blk0 + g - 31) < j1) j1 = N - (blk0 + g - 31);
             float a0 = 0.f, a1 = 0.f;
+#pragma unroll 8
             for (int j = 0; j < 32; ++j) {
-                const int i = g - 31 + j, key = k0 + t * 32 + j;
-                if (i >= 0 && i < nq32 && p + j >= 0 && key >= prefix && blk0 + i < N && key < N) {
-                    const float v = S[i * 33 + j];
-                    if (x >= dx) a0 += v; else a1 += v;
-                }
+                const bool in = j >= j0 && j < j1;
+                const float v = S[in ? (g - 31) * 33 + j * 34 : 0];
+                a0 += in && x >= dx ? v : 0.f;
+                a1 += in && x < dx ? v : 0.f;
                 x = x + 1 == gw ? 0 : x + 1;
             }
             const int v = g + 32 * (KT - 1 - t);
@@ -545,12 +561,12 @@ int plan_workspace(const vit_rel_pos* pos, int batch, int heads, int head_dim, W
     VIT_TRY_RC(vit_cu_count(&ncu));
     const int N = pos->prefix + pos->grid_h * pos->grid_w, n32 = ceil_div(N, 32);
     // query blocks of up to 8 waves, all alike; key blocks of 7 tiles where that is the whole sequence (one block: Q, dO, K, V are read
-    // once a sample) and the head dim leaves the registers room for it, else 4 tiles, 2 where the expansion of a long sequence
-    // leaves the images less
+    // once a sample) and the head dim leaves the registers room for it (a spilled register's reload waits for all loads under
+    // way), else 4 tiles, 2 for head_dim 128 and where the expansion of a long sequence leaves the images less
     w->tq = ceil_div(n32, 8);
     w->bq = ceil_div(n32, w->tq) * 32;
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, w->bq);
-    w->bk = (head_dim <= 64 && n32 > 4 && n32 <= 7 ? 7 : bias_lds(head_dim, 4, slice) <= 160 * 1024 ? 4 : 2) * 32;
+    w->bk = (head_dim <= 64 && n32 > 4 && n32 <= 7 ? 7 : head_dim <= 112 && bias_lds(head_dim, 4, slice) <= 160 * 1024 ? 4 : 2) * 32;
     w->tk = ceil_div(N, w->bk);
     w->fp = 2 * (w->bq + w->bk - 1) + 4;
     // enough sample ranges to give every CU a workgroup, whole samples each
@@ -587,11 +603,15 @@ int launch_bias_grad(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t st
 
 template <int DH>
 int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
-    VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, stream)));
-    VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, stream)));
+    if (attention_rel_bwd_dh64_eligible(a.N, a.H, a.HK, DH)) {
+        VIT_TRY_RC(launch_attention_rel_bwd_dh64(a.geo, a.qkv, a.out, a.dout, a.lse, a.delta, a.dqkv, a.lengths, a.B, a.N, a.H, a.scale, stream));
+    } else {
+        VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, stream)));
+        VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, stream)));
+    }
     if (!a.dtable) return VIT_OK;
     if (a.bk == 7 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 64 ? 7 : 4)>(a, pos, stream)));
-    else if (a.bk == 4 * 32) VIT_TRY_RC((launch_bias_grad<DH, 4>(a, pos, stream)));
+    else if (a.bk == 4 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 112 ? 4 : 2)>(a, pos, stream)));
     else VIT_TRY_RC((launch_bias_grad<DH, 2>(a, pos, stream)));
     const int total = a.geo.offsets + (a.geo.prefix ? 3 : 0);
     // without a map, and with nothing in the table behind the offsets, the offset sums are the table's gradient

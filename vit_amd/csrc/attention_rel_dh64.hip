@@ -123,18 +123,15 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
 
     // ---- prologue: the expansion of the first item's head, then Q of item 0 and the first R - 1 tiles
     Item cur = item_at(0);
-    int slice_n = 0;
-    int qcode = 0;  // code of the lane's query + center - first offset of the slice
+    RelLane<true> rl;
     auto expand = [&](const Item& t) {  // all threads, between barriers
         const int blk0 = t.qb * NW * 32;
         const int blk1 = blk0 + NW * 32 < N ? blk0 + NW * 32 - 1 : N - 1;
         const RelSlice sl(a.geo, blk0, blk1, true);
-        rel_expand(a.geo, T, sl.lo, sl.n, t.h);
-        slice_n = sl.n;
-        const int q = blk0 + wave * 32 + r;
-        qcode = rel_code(a.geo, q < N ? q : N - 1) + a.geo.center - sl.lo;
+        rel_expand(a.geo, T, sl, true, t.h);
+        for (int i = tid; i < nt * 32; i += NW * 64) codes[i] = rel_row_code(a.geo, sl, true, i);
+        rl = RelLane<true>(a.geo, sl, T, blk0 + wave * 32 + r, N - 1);
     };
-    for (int i = tid; i < nt * 32; i += NW * 64) codes[i] = rel_code(a.geo, i);
     expand(cur);
     wait_vm<0>();  // (the expansion's own loads: the counted waits below start from none outstanding)
     __syncthreads();
@@ -196,7 +193,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
             const unsigned kb_lds = smem_lds + (unsigned)(slot * SLOT);
             const int key0 = p * 32;
             f32x16 s;
-            rel_tile<true>(s, T, codes + key0, qcode, hi, a.geo.prefix, slice_n, q0 + r, key0);
+            rel_tile(s, codes + key0, rl, hi, a.geo.prefix, key0);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 const bf16x8 kf = *(const bf16x8*)(Kb + kro[ks]);

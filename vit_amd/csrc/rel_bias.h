@@ -33,60 +33,94 @@ __device__ __forceinline__ float rel_entry(const RelGeo& g, int index, int head)
     const float v = g.table[(size_t)b * g.heads + head];
     return v < kRelMasked ? -INFINITY : v * g.inv_scale;
 }
-// The block of LDS that one head's product tiles start from: entries lo .. lo + n - 1 of the offsets, then the three prefix
-// entries. All threads of the workgroup.
-__device__ __forceinline__ void rel_expand(const RelGeo& g, float* T, int lo, int n, int head) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) T[i] = rel_entry(g, lo + i, head);
-    if (g.prefix && threadIdx.x < 3) T[n + threadIdx.x] = rel_entry(g, g.offsets + threadIdx.x, head);
-}
-// The slice that the queries first .. last of a block reach over all keys (QUERY), or the keys first .. last over all queries.
-// lane_add / row_add make an index into it: query code + .. - key code, both sides' constant on the lane (QLANE) or the row.
+// The slice of offsets that the queries first .. last of a block reach over all keys (query), or the keys first .. last over all
+// queries: entries lo .. lo + n - 1. Behind it in LDS, with a prefix: span + 1 copies of the entry of a prefix token on the other side,
+// which that token's made-up code addresses like an offset (so it needs no test), the entry of a prefix token on the block's side, and
+// that of a pair of them.
 struct RelSlice {
-    int lo, n;
-    __device__ RelSlice(const RelGeo& g, int first, int last, bool query) {
-        const int c0 = rel_code(g, first), c1 = rel_code(g, last), cmax = rel_code(g, g.prefix + g.grid - 1);
+    int lo, n, span, c0, c1;
+    __device__ RelSlice(const RelGeo& g, int first, int last, bool query) {  // uniform arguments: kept in scalar registers
+        c0 = __builtin_amdgcn_readfirstlane(rel_code(g, first));
+        c1 = __builtin_amdgcn_readfirstlane(rel_code(g, last));
+        const int cmax = __builtin_amdgcn_readfirstlane(rel_code(g, g.prefix + g.grid - 1));
         lo = (query ? c0 - cmax : -c1) + g.center;
-        n = c1 - c0 + cmax + 1;
+        span = c1 - c0;
+        n = span + cmax + 1;
     }
 };
+// All threads of the workgroup.
+__device__ __forceinline__ void rel_expand(const RelGeo& g, float* T, const RelSlice& s, bool query, int head) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (opaque: nothing of this is worth a register in the loops around it)
+    for (int i = tid; i < s.n; i += blockDim.x) T[i] = rel_entry(g, s.lo + i, head);
+    if (g.prefix) {
+        const float other = rel_entry(g, g.offsets + (query ? 1 : 0), head);
+        for (int i = tid; i <= s.span; i += blockDim.x) T[s.n + i] = other;
+        if (tid < 2) T[s.n + s.span + 1 + tid] = rel_entry(g, g.offsets + (tid ? 2 : query ? 0 : 1), head);
+    }
+}
+// 4 * code of a row's token, rows being the side that is not the block's
+__device__ __forceinline__ int rel_row_code(const RelGeo& g, const RelSlice& s, bool query, int token) {
+    if (token < g.prefix) return 4 * (query ? s.c0 + g.center - s.lo - s.n : s.n + s.c1 - g.center + s.lo);
+    return 4 * rel_code(g, token);
+}
 
 // Start values of a 32 x 32 product tile whose register e is row row0 + (e & 3) + 8 (e >> 2) + 4 hi and whose lane is the column.
-// QLANE: the lane is the query (rows are keys): index = lane_code - code; otherwise index = code - lane_code, where either the
-// lane's or the rows' codes already hold center - lo. `codes`: the 32 rows' codes in LDS; n: the slice's length.
+// Everything is in bytes, so that an entry costs one subtraction and one read: `codes` are the 32 rows' codes in LDS; QLANE (the lane
+// is the query, rows are keys): an entry is at `at` - code, otherwise at `at` + code.
+typedef __attribute__((address_space(3))) const float* lds_float;
+__device__ __forceinline__ int rel_lds(const float* T) { return (int)(uintptr_t)LDS_PTR((void*)T); }
 template <bool QLANE>
-__device__ __forceinline__ void rel_tile(f32x16& s, const float* T, const int* codes, int lane_code, int hi, int prefix, int n, int lane_tok,
-                                         int row0) {
+struct RelLane {
+    int at, mask, both;  // mask: 0 on a lane with a prefix token (`at` is then its entry, whatever the row); both: address of the pair's entry
+    bool any;            // wave-uniform: the wave has such lanes
+    __device__ RelLane() {}
+    __device__ RelLane(const RelGeo& g, const RelSlice& s, const float* T, int token, int last) {
+        const bool lp = token < g.prefix;
+        const int c = rel_code(g, token < last ? token : last);
+        at = rel_lds(T) + 4 * (lp ? s.n + s.span + 1 : g.center - s.lo + (QLANE ? c : -c));
+        mask = lp ? 0 : -1;
+        both = __builtin_amdgcn_readfirstlane(rel_lds(T) + 4 * (s.n + s.span + 2));
+        any = __any(lp);
+    }
+};
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+// the rows' codes into registers, and with them the start values (two steps: a pipelined loop puts other work between them)
+__device__ __forceinline__ void rel_codes(i32x16& c, const int* codes, int hi) {
     typedef int i32x4 __attribute__((ext_vector_type(4)));
-    if (row0 < prefix || __any(lane_tok < prefix)) {  // wave-uniform: only tiles that hold a prefix token
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+        const i32x4 v = *(const i32x4*)(codes + 8 * g4 + 4 * hi);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[g4 * 4 + j] = v[j];
+    }
+}
+template <bool QLANE>
+__device__ __forceinline__ void rel_start(f32x16& s, const i32x16& c, const RelLane<QLANE>& l, int hi, int prefix, int row0) {
+    if (l.any) {
         int lim = prefix - row0 - 4 * hi;
         asm volatile("" : "+v"(lim));  // (opaque: 16 lane masks would be hoisted into 32 SGPRs)
-        const bool lp = lane_tok < prefix;
-        const int one = n + (lp ? (QLANE ? 0 : 1) : (QLANE ? 1 : 0));  // entry of a pair with a prefix row / without, by the lane's side
+        if (l.mask) lim = -64;
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-            const i32x4 c = *(const i32x4*)(codes + 8 * g4 + 4 * hi);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool rp = 8 * g4 + j < lim;
-                int at = QLANE ? lane_code - c[j] : c[j] - lane_code;
-                at = lp || rp ? one : at;
-                at = lp && rp ? n + 2 : at;
-                s[g4 * 4 + j] = T[at];
-            }
+        for (int e = 0; e < 16; ++e) {
+            const int m = c[e] & l.mask, at = QLANE ? l.at - m : l.at + m;
+            s[e] = *(lds_float)(uintptr_t)((e & 3) + 8 * (e >> 2) < lim ? l.both : at);
         }
     } else {
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-            const i32x4 c = *(const i32x4*)(codes + 8 * g4 + 4 * hi);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[g4 * 4 + j] = T[QLANE ? lane_code - c[j] : c[j] - lane_code];
-        }
+        for (int e = 0; e < 16; ++e) s[e] = *(lds_float)(uintptr_t)(QLANE ? l.at - c[e] : l.at + c[e]);
     }
+}
+template <bool QLANE>
+__device__ __forceinline__ void rel_tile(f32x16& s, const int* codes, const RelLane<QLANE>& l, int hi, int prefix, int row0) {
+    i32x16 c;
+    rel_codes(c, codes, hi);
+    rel_start(s, c, l, hi, prefix, row0);
 }
 
 // ---- host side
 // Largest slice of offsets that a block of `block` consecutive tokens needs: all codes of the other side plus its own span
-// (floats, with the three prefix entries)
+// (floats, with what stands behind the slice)
 static inline int rel_slice_max(int gh, int gw, int block) {
     const int grid = gh * gw;
     const int max_code = (gh - 1) * (2 * gw - 1) + gw - 1;
@@ -94,7 +128,7 @@ static inline int rel_slice_max(int gh, int gw, int block) {
     // a block that starts in column x > 0 spans one row border more than one that starts at 0
     int span = last + ((last + gw - 1) / gw) * (gw - 1);
     if (span > max_code) span = max_code;
-    return max_code + span + 1 + 3;
+    return max_code + 2 * span + 4;
 }
 constexpr int kRelSliceCap = 16384;  // floats: 64 KiB of LDS
 int rel_make_geo(const char* who, const vit_rel_pos* pos, const float* table, int heads, float scale, RelGeo* out, int* seq);
