@@ -4,6 +4,7 @@
 //
 // Beyond attention.hip: per-sample lengths (keys behind them are never read, queries behind them give zeros), key / value
 // heads shared by groups of query heads, entries that mask (a query whose every key is masked gives zeros and lse = +inf).
+#include "lds_image.h"
 #include "rel_bias.h"
 #include <math.h>
 
@@ -17,18 +18,15 @@ struct RelFwdArgs {
     float* lse;
     const int* lengths;
     RelGeo geo;
-    int N, H, HK, KC, slice;  // slice: floats of LDS for the expansion
+    int N, H, HK, KC;
     float scale_log2e;
 };
 
-template <int DH>
-struct RGeo {
-    static constexpr int KSTEPS = DH / 16;
-    static constexpr int DB = (DH + 31) / 32;
-    static constexpr int KS = DH * 2 + 16;     // K row stride, bytes
-    static constexpr int VS = (DB | 1) * 64;   // V row stride, bytes (odd multiple of 64)
-    static constexpr int CHUNKS = DH / 8;
-};
+constexpr float kDeferLog2 = 6.0f;  // the running max is left alone until a score outgrows it by more than this (base 2)
+constexpr float kFloor = -1e35f;    // a running max never falls below this: masked scores (-inf) then have probability 0
+constexpr int KCH = 32;             // keys of a staged chunk
+// waves of a workgroup: with two workgroups a CU (their LDS fits twice) as many as the head dim's registers allow, 4, 3 or 2 a SIMD
+constexpr int rel_waves(int dh) { return 4; }
 
 __device__ __forceinline__ bf16x8 pack8(const f32x16& p, int s) {
     bf16x8 o;
@@ -42,123 +40,130 @@ __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
     return n < 0 ? 0 : n > N ? N : n;
 }
 
+// bf16, any head dim and length. A workgroup of up to 4 waves takes 32 queries a wave of one (sample, head); keys and values come in chunks
+// of 64 by LDS-DMA into two buffers, the next chunk under the products of this one: one barrier a chunk, and two or three workgroups a CU
+// to fill what a wave waits for (a few rows of LDS per workgroup, against whole sequences staged at once: ... ).
 template <int DH>
-__global__ __launch_bounds__(512) void attention_rel_bf16_kernel(const RelFwdArgs a) {
-    using G = RGeo<DH>;
+__global__ __launch_bounds__(64 * rel_waves(DH)) __attribute__((amdgpu_waves_per_eu(DH <= 64 ? 4 : 3))) void attention_rel_bf16_kernel(const RelFwdArgs a) {
+    using I = LdsImage<DH>;
+    constexpr int KS = DH / 16, DB = (DH + 31) / 32, IMG = KCH * I::ROW;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int KC = a.KC, N = a.N, H = a.H;
-    unsigned char* Kl = smem;
-    unsigned char* Vl = smem + (size_t)KC * G::KS;
-    int* codes = (int*)(Vl + (size_t)KC * G::VS);
-    float* T = (float*)(codes + KC);
+    const int N = a.N, H = a.H;
+    int* const codes = (int*)(smem + 4 * IMG);  // [2][KCH]; images: [2][K, V]
+    float* const T = (float*)(codes + 2 * KCH);
+    const unsigned lds0 = (unsigned)(uintptr_t)LDS_PTR(smem);
 
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nwaves = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
     const int r = lane & 31, hi = lane >> 5;
     const int b = blockIdx.x / H, h = blockIdx.x - b * H, hk = h / (H / a.HK);
-    const size_t rs = (size_t)(H + 2 * a.HK) * DH;
-    const bf16_t* base = (const bf16_t*)a.qkv + (size_t)b * N * rs;
-    const bf16_t* kbase = base + (size_t)(H + hk) * DH;
-    const bf16_t* vbase = kbase + (size_t)a.HK * DH;
-    const int nb = sample_length(a.lengths, b, N);
-
-    const int blk0 = blockIdx.y * nwaves * 32;
+    const int pitch = (H + 2 * a.HK) * DH * 2;
+    const unsigned char* base = (const unsigned char*)a.qkv + (size_t)b * N * pitch;
+    const int nb = __builtin_amdgcn_readfirstlane(sample_length(a.lengths, b, N));
+    const int blk0 = (gridDim.y - 1 - blockIdx.y) * nw * 32, blk1 = blk0 + nw * 32 - 1;  // (last blocks first: only long samples have them)
     const int q0 = blk0 + wave * 32, q = q0 + r;
-    const int qrow = q < nb ? q : (nb > 0 ? nb - 1 : 0);
-    bf16x8 qf[G::KSTEPS];
-#pragma unroll
-    for (int ks = 0; ks < G::KSTEPS; ++ks) qf[ks] = *(const bf16x8*)(base + (size_t)qrow * rs + (size_t)h * DH + ks * 16 + hi * 8);
+    const int nc = blk0 < nb ? (nb + KCH - 1) / KCH : 0;  // (a block of rows behind the sample only stores zeros)
 
-    const int blk1 = blk0 + nwaves * 32 - 1;
+    const __amdgpu_buffer_rsrc_t kr = head_resource<DH>(base + (size_t)(H + hk) * DH * 2, N, pitch);
+    const __amdgpu_buffer_rsrc_t vr = head_resource<DH>(base + (size_t)(H + a.HK + hk) * DH * 2, N, pitch);
     const RelSlice sl(a.geo, blk0, blk1 < N ? blk1 : N - 1, true);
+    auto stage = [&](int c) {
+        unsigned char* const dst = smem + (c & 1) * 2 * IMG;
+        // whole tiles up to the sample's last key (rows behind it re-read that key: what is masked is still finite)
+        const int need = nb - c * KCH < KCH ? (nb - c * KCH + 31) & ~31 : KCH;
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // (opaque: the lane offsets are made here, not kept in registers over the products)
+        for (int i = wave * I::RPI; i < need; i += nw * I::RPI) {
+            I::dma(kr, dst, i, KCH, c * KCH, nb - 1, pitch, ln);
+            I::dma(vr, dst + IMG, i, KCH, c * KCH, nb - 1, pitch, ln);
+        }
+        for (int i = tid; i < KCH; i += blockDim.x) codes[(c & 1) * KCH + i] = rel_row_code(a.geo, sl, true, c * KCH + i);
+    };
+    if (nc > 0) stage(0);
+    bf16x8 qf[KS];
+    {
+        const int qrow = q < nb ? q : (nb > 0 ? nb - 1 : 0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const bf16x8*)(base + (size_t)qrow * pitch + (size_t)h * DH * 2 + ks * 32 + hi * 16);
+    }
     rel_expand(a.geo, T, sl, true, h);
     const RelLane<true> rl(a.geo, sl, T, q, N - 1);
+    const TrRead<DH> tr(lane);
+    const int ro = (int)lds0 + I::at(r, hi);
 
-    f32x16 o[G::DB];
+    f32x16 o[DB];
 #pragma unroll
-    for (int d = 0; d < G::DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
-
-    const int g = lane >> 4, i16 = lane & 15;
-    const int tr_key = 4 * (g >> 1) + (i16 >> 2);
-    const int tr_col = ((g & 1) * 16 + 4 * (i16 & 3)) * 2;
-
-    for (int kc0 = 0; kc0 < nb; kc0 += KC) {
-        int nkeys = nb - kc0;
-        nkeys = nkeys > KC ? KC : (nkeys + 31) & ~31;
-        __syncthreads();
-        const int total = nkeys * G::CHUNKS;
-        for (int idx = tid; idx < total; idx += blockDim.x) {
-            const int key = idx / G::CHUNKS, c = idx - key * G::CHUNKS;
-            int gk = kc0 + key;
-            if (gk > nb - 1) gk = nb - 1;  // pad keys re-read the last row (their scores are masked)
-            *(bf16x8*)(Kl + (size_t)key * G::KS + c * 16) = *(const bf16x8*)(kbase + (size_t)gk * rs + c * 8);
-            *(bf16x8*)(Vl + (size_t)key * G::VS + c * 16) = *(const bf16x8*)(vbase + (size_t)gk * rs + c * 8);
-        }
-        for (int i = tid; i < nkeys; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, kc0 + i);
-        __syncthreads();
-
-        for (int t = 0; t < nkeys >> 5; ++t) {
-            const int key0 = kc0 + t * 32;
+    float m_run = kFloor, l_run = 0.f;
+    for (int c = 0; c < nc; ++c) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");  // the chunk is whole; nobody reads the other buffer any more
+        if (c + 1 < nc) stage(c + 1);
+        const int img = (c & 1) * 2 * IMG;
+#pragma unroll 1
+        for (int t = 0; t < KCH / 32; ++t) {
+            const int key0 = c * KCH + t * 32;
+            if (key0 >= nb) break;
             f32x16 s;
-            rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
-            const unsigned char* kp = Kl + (size_t)(t * 32 + r) * G::KS + hi * 16;
+            rel_tile(s, codes + (c & 1) * KCH + t * 32, rl, hi, a.geo.prefix, key0);
+            int ka = ro + img + t * 32 * I::ROW;
+            asm volatile("" : "+v"(ka));
 #pragma unroll
-            for (int ks = 0; ks < G::KSTEPS; ++ks)
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kp + ks * 32), qf[ks], s, 0, 0, 0);
+            for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks)), qf[ks], s, 0, 0, 0);
+            const unsigned vimg = lds0 + (unsigned)(img + IMG + t * 32 * I::ROW);
+            bf16x8 vt[2][DB];
+            if constexpr (DB == 4) tr.template read_step<0>(vt[0], vimg);  // (32 registers at once would cost a wave a SIMD)
+            else tr.read(vt, vimg);
             if (key0 + 32 > nb) {
+                int lim = nb - key0 - 4 * hi;
+                asm volatile("" : "+v"(lim));  // (opaque: the 16 lane masks would be hoisted into 32 SGPRs)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (key0 + (e & 3) + 8 * (e >> 2) + 4 * hi >= nb) s[e] = -INFINITY;
+                    if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
             }
             float mx = s[0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
             mx = max_across_halves(mx);
+            // rescale only when a score outgrows the running max by more than kDeferLog2: P stays <= 2^kDeferLog2 until then
             const float m_new = fmaxf(m_run, mx * a.scale_log2e);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;  // nothing but masked keys so far
-            const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-            m_run = m_new;
-            float psum = 0.f;
+            if (__any(m_new > m_run + kDeferLog2)) {
+                const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                l_run *= alpha;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - m_use);
-                psum += s[e];
-            }
-            l_run = l_run * alpha + psum;
-            if (__any(alpha != 1.f)) {
-#pragma unroll
-                for (int d = 0; d < G::DB; ++d)
+                for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
             }
+            float psum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - m_run);
+                psum += s[e];
+            }
+            l_run += psum;
 #pragma unroll
             for (int sk = 0; sk < 2; ++sk) {
+                if constexpr (DB == 4)
+                    if (sk == 1) tr.template read_step<1>(vt[1], vimg);
                 const bf16x8 pb = pack8(s, sk);
-                const unsigned char* vp = Vl + (size_t)(t * 32 + 16 * sk + tr_key) * G::VS + tr_col;
 #pragma unroll
-                for (int d = 0; d < G::DB; ++d) {
-                    const short4v lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(vp + d * 64));
-                    const short4v hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(vp + 8 * G::VS + d * 64));
-                    const short8v both = __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, both), pb, o[d], 0, 0, 0);
-                }
+                for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt[sk][d], pb, o[d], 0, 0, 0);
             }
         }
     }
 
     const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-    const bool any = l_tot > 0.f || l_tot != l_tot;  // (a NaN row stays one)
-    const bool live = q < nb && any;
+    const bool live = q < nb && (l_tot > 0.f || l_tot != l_tot);  // (a NaN row stays one)
     const float inv = 1.0f / l_tot;
     if (q < N) {
         if (a.lse != nullptr && hi == 0) a.lse[((size_t)b * H + h) * N + q] = live ? m_run + log2f(l_tot) : INFINITY;
         const size_t at = ((size_t)b * N + q) * H * DH + (size_t)h * DH;
 #pragma unroll
-        for (int d = 0; d < G::DB; ++d)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int d0 = d * 32 + 8 * g4 + 4 * hi;
@@ -308,26 +313,41 @@ int pick_waves(int N, int* qblocks) {
 }
 
 template <int DH>
-int launch_rel(RelFwdArgs a, const vit_rel_pos* pos, int batch, int dtype, hipStream_t stream) {
+int launch_rel_bf16(RelFwdArgs a, const vit_rel_pos* pos, int batch, hipStream_t stream) {
+    const int n32 = ceil_div(a.N, 32), qblocks = ceil_div(n32, rel_waves(DH)), waves = ceil_div(n32, qblocks);  // equal blocks
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
+    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
+    const size_t lds = (size_t)4 * KCH * LdsImage<DH>::ROW + (size_t)(2 * KCH + slice) * 4;
+    static PerDeviceInt attr_set;
+    std::atomic<int>* as = attr_set.slot();
+    if (!as || !as->load(std::memory_order_relaxed)) {
+        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)attention_rel_bf16_kernel<DH>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (as) as->store(1, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(attention_rel_bf16_kernel<DH>, dim3(batch * a.H, qblocks), dim3(waves * 64), lds, stream, a);
+    VIT_CHECK_HIP(hipGetLastError());
+    return VIT_OK;
+}
+
+template <int DH>
+int launch_rel_f32(RelFwdArgs a, const vit_rel_pos* pos, int batch, hipStream_t stream) {
     int qblocks;
     const int waves = pick_waves(a.N, &qblocks);
-    const int per_key = dtype == VIT_BF16 ? RGeo<DH>::KS + RGeo<DH>::VS + 4 : (DH + 1 + (DH + 31) / 32 * 32 + 1) * 4;
-    a.slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
-    VIT_REQUIRE(a.slice <= kRelSliceCap, "attention_rel: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, a.slice, kRelSliceCap);
+    const int per_key = (DH + 1 + (DH + 31) / 32 * 32 + 1) * 4;
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
+    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     int KC = 80 * 1024 / per_key / 32 * 32;
     const int npad = (a.N + 31) / 32 * 32;
     if (KC > npad) KC = npad;
     a.KC = KC;
-    const size_t lds = (size_t)KC * per_key + (size_t)a.slice * 4;
-    const void* kern = dtype == VIT_BF16 ? (const void*)attention_rel_bf16_kernel<DH> : (const void*)attention_rel_f32_kernel<DH>;
-    static PerDeviceInt attr_set[2];
-    std::atomic<int>* as = attr_set[dtype].slot();
+    const size_t lds = (size_t)KC * per_key + (size_t)slice * 4;
+    static PerDeviceInt attr_set;
+    std::atomic<int>* as = attr_set.slot();
     if (!as || !as->load(std::memory_order_relaxed)) {
-        VIT_CHECK_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)attention_rel_f32_kernel<DH>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (as) as->store(1, std::memory_order_relaxed);
     }
-    if (dtype == VIT_BF16) hipLaunchKernelGGL(attention_rel_bf16_kernel<DH>, dim3(batch * a.H, qblocks), dim3(waves * 64), lds, stream, a);
-    else hipLaunchKernelGGL(attention_rel_f32_kernel<DH>, dim3(batch * a.H, qblocks), dim3(waves * 64), lds, stream, a);
+    hipLaunchKernelGGL(attention_rel_f32_kernel<DH>, dim3(batch * a.H, qblocks), dim3(waves * 64), lds, stream, a);
     VIT_CHECK_HIP(hipGetLastError());
     return VIT_OK;
 }
@@ -374,10 +394,11 @@ extern "C" int vit_attention_rel_fwd(const vit_rel_pos* pos, const void* qkv, co
     a.H = heads;
     a.HK = kv_heads;
     a.scale_log2e = scale * LOG2E;
+    VIT_REQUIRE((int64_t)a.N * (heads + 2 * kv_heads) * head_dim * (dtype == VIT_BF16 ? 2 : 4) < (1LL << 31), "vit_attention_rel_fwd: one sample's qkv rows exceed 2 GiB");
     if (dtype == VIT_BF16 && head_dim == 64 && !lengths && attention_rel_dh64_eligible(pos, batch, heads, kv_heads))
         return launch_attention_rel_dh64(pos, a.geo, qkv, out, lse, batch, heads, kv_heads, scale, (hipStream_t)stream);
 #define REL_CASE(DHV) \
-    case DHV: return launch_rel<DHV>(a, pos, batch, dtype, (hipStream_t)stream);
+    case DHV: return dtype == VIT_BF16 ? launch_rel_bf16<DHV>(a, pos, batch, (hipStream_t)stream) : launch_rel_f32<DHV>(a, pos, batch, (hipStream_t)stream);
     switch (head_dim) {
         REL_CASE(16) REL_CASE(32) REL_CASE(48) REL_CASE(64) REL_CASE(80) REL_CASE(96) REL_CASE(112) REL_CASE(128)
     }

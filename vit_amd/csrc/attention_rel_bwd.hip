@@ -22,7 +22,7 @@
 
 // launches 1 and 2 in one pass where a head fits the LDS (attention_rel_bwd_dh64.hip)
 bool attention_rel_bwd_dh64_eligible(int N, int heads, int kv_heads, int head_dim);
-int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,
+int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* ndelta, void* dqkv,
                                   const int* lengths, int batch, int N, int heads, float scale, hipStream_t stream);
 
 namespace {
@@ -35,7 +35,7 @@ struct RelBwdArgs {
     const bf16_t* out;
     const bf16_t* dout;
     const float* lse;
-    float* delta;  // [B, H, N]
+    float* ndelta;  // [B, H, N]: -delta, the start value of dP's products
     bf16_t* dqkv;
     float* part;   // [splits][H][tq][tk][fp]: folded sums of the blocks
     float* doff;   // [H][offsets + 3] (with a map)
@@ -44,18 +44,9 @@ struct RelBwdArgs {
     const int* bucket_start;
     const int* lengths;
     RelGeo geo;
-    int B, N, H, HK, IC;
+    int B, N, H, HK;
     int splits, tq, tk, bq, bk, fp;  // bias gradient: sample ranges, query / key blocks, their sizes, pitch of their sums
     float scale, scale_log2e;
-};
-
-template <int DH>
-struct BGeo {
-    static constexpr int KSTEPS = DH / 16;
-    static constexpr int DB = (DH + 31) / 32;
-    static constexpr int RS = DH * 2 + 16;     // row-read image stride, bytes
-    static constexpr int TS = (DB | 1) * 64;   // transposed-read image stride, bytes
-    static constexpr int CHUNKS = DH / 8;
 };
 
 __device__ __forceinline__ bf16x8 pack8b(const f32x16& p, int s) {
@@ -64,184 +55,200 @@ __device__ __forceinline__ bf16x8 pack8b(const f32x16& p, int s) {
     for (int e = 0; e < 8; ++e) o[e] = (bf16_t)p[8 * s + e];
     return o;
 }
-template <int TS>
-__device__ __forceinline__ bf16x8 tr_frag(const unsigned char* img, int row0, int sk, int d, int tr_key, int tr_col) {
-    const unsigned char* vp = img + (size_t)(row0 + 16 * sk + tr_key) * TS + tr_col + d * 64;
-    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(vp));
-    const short4v hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(vp + 8 * TS));
-    const short8v both = __builtin_shufflevector(lo, hi4, 0, 1, 2, 3, 4, 5, 6, 7);
-    return __builtin_bit_cast(bf16x8, both);
-}
 __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
     if (!lengths) return N;
     const int n = lengths[b];
     return n < 0 ? 0 : n > N ? N : n;
 }
 
+// what the registers allow without a spill (a spilled register's reload waits for all loads under way)
+constexpr int bwd_waves_per_simd(int dh, int mode) { return mode == MODE_DQ ? (dh <= 96 ? 3 : 2) : dh <= 64 ? 3 : dh <= 96 ? 2 : 1; }
+// A workgroup of up to 4 waves takes 32 outer rows a wave of one (sample, head); the inner rows come in chunks of 32 by LDS-DMA into two
+// buffers, the next chunk under the products of this one, in images that serve row reads and transposed reads alike.
 template <int DH, int MODE>
-__global__ __launch_bounds__(512) void attn_rel_bwd_kernel(const RelBwdArgs a) {
-    using G = BGeo<DH>;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_per_simd(DH, MODE)))) void attn_rel_bwd_kernel(const RelBwdArgs a) {
+    using I = LdsImage<DH>;
+    constexpr int KS = DH / 16, DB = (DH + 31) / 32, CR = 32, IMG = CR * I::ROW;
+    constexpr int BUF = 2 * IMG + (MODE == MODE_DKV ? 512 : 256);  // two images, (lse, -delta), codes; a multiple of 256 (LdsImage::step)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int IC = a.IC, N = a.N, H = a.H, HK = a.HK;
-    unsigned char* R1 = smem;                        // [IC][RS] K (DQ) / Q (DKV)
-    unsigned char* R2 = R1 + (size_t)IC * G::RS;     // [IC][RS] V (DQ) / dO (DKV)
-    unsigned char* T1 = R2 + (size_t)IC * G::RS;     // [IC][TS] transposed-read image of R1
-    unsigned char* T2 = T1 + (size_t)IC * G::TS;     // of R2 (DKV)
-    float* rowL = (float*)(T2 + (MODE == MODE_DKV ? (size_t)IC * G::TS : 0));  // [IC] (DKV)
-    float* rowD = rowL + (MODE == MODE_DKV ? IC : 0);                          // [IC] (DKV)
-    int* codes = (int*)(rowD + (MODE == MODE_DKV ? IC : 0));                   // [IC]
-    float* T = (float*)(codes + IC);
-
+    float* const T = (float*)(smem + 2 * BUF);
+    const int lds0 = (int)(uintptr_t)LDS_PTR(smem);
+    const int N = a.N, H = a.H, HK = a.HK;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nwaves = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
     const int r = lane & 31, hi = lane >> 5;
     const int OH = MODE == MODE_DQ ? H : HK;  // outer heads
     const int b = blockIdx.x / OH, oh = blockIdx.x - b * OH, group = H / HK;
-    const size_t rs = (size_t)(H + 2 * HK) * DH, os = (size_t)H * DH;
-    const int g = lane >> 4, i16 = lane & 15;
-    const int tr_key = 4 * (g >> 1) + (i16 >> 2);
-    const int tr_col = ((g & 1) * 16 + 4 * (i16 & 3)) * 2;
-    const int nb = sample_length(a.lengths, b, N);
-    const int blk0 = blockIdx.y * nwaves * 32;
-    const int blk1 = min(blk0 + nwaves * 32, N) - 1;
+    const int pitch = (H + 2 * HK) * DH * 2, opitch = H * DH * 2;
+    const int nb = __builtin_amdgcn_readfirstlane(sample_length(a.lengths, b, N));
+    const int blk0 = (gridDim.y - 1 - blockIdx.y) * nw * 32;  // (last blocks first: only long samples have them)
+    const int blk1 = min(blk0 + nw * 32, N) - 1;
     const int o0 = blk0 + wave * 32, row = o0 + r;
-    const int orow = row < nb ? row : (nb > 0 ? nb - 1 : 0);
-    const bf16_t* base = a.qkv + (size_t)b * N * rs;
+    const unsigned char* base = (const unsigned char*)a.qkv + (size_t)b * N * pitch;
+    const unsigned char* gbase = (const unsigned char*)a.dout + (size_t)b * N * opitch;
     const int hk = MODE == MODE_DQ ? oh / group : oh;
-    const bf16_t* kbase = base + (size_t)(H + hk) * DH;
-    const bf16_t* vbase = kbase + (size_t)HK * DH;
+    const int nheads = MODE == MODE_DQ ? 1 : group;
+    const int nc = blk0 < nb ? (nb + CR - 1) / CR : 0, steps = nc * nheads;
+    const RelSlice sl(a.geo, blk0, blk1, MODE == MODE_DQ);  // over all keys / all queries
+
+    auto stage = [&](int step) {
+        const int gh = step / nc, c = step - gh * nc, h = MODE == MODE_DQ ? oh : oh * group + gh, row0 = c * CR;
+        unsigned char* const dst = smem + (step & 1) * BUF;
+        // rows behind the sample re-read its last one: what is masked is still finite
+        const __amdgpu_buffer_rsrc_t r1 = head_resource<DH>(base + (size_t)(MODE == MODE_DQ ? H + hk : h) * DH * 2, N, pitch);
+        const __amdgpu_buffer_rsrc_t r2 = MODE == MODE_DQ ? head_resource<DH>(base + (size_t)(H + HK + hk) * DH * 2, N, pitch)
+                                                          : head_resource<DH>(gbase + (size_t)h * DH * 2, N, opitch);
+        int ln = lane;
+        asm volatile("" : "+v"(ln));  // (opaque: the lane offsets are made here, not kept in registers over the products)
+        for (int i = wave * I::RPI; i < CR; i += nw * I::RPI) {
+            I::dma(r1, dst, i, CR, row0, nb - 1, pitch, ln);
+            I::dma(r2, dst + IMG, i, CR, row0, nb - 1, MODE == MODE_DQ ? pitch : opitch, ln);
+        }
+        if constexpr (MODE == MODE_DKV) {
+            if (wave == 0) {  // the queries' lse and -delta
+                const size_t at = ((size_t)b * H + h) * N;
+                int q = row0 + ln;
+                q = q < nb ? q : nb - 1;
+                const __amdgpu_buffer_rsrc_t rl_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.lse + at), 0, (unsigned)N * 4, 0x00020000);
+                const __amdgpu_buffer_rsrc_t rd_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.ndelta + at), 0, (unsigned)N * 4, 0x00020000);
+                if (ln < CR) {
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rl_, LDS_PTR(dst + 2 * IMG), 4, q * 4, 0, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rd_, LDS_PTR(dst + 2 * IMG + CR * 4), 4, q * 4, 0, 0, 0);
+                }
+            }
+        }
+        if (ln < CR && wave == nw - 1) *(int*)(dst + BUF - CR * 4 + ln * 4) = rel_row_code(a.geo, sl, MODE == MODE_DQ, row0 + ln);
+    };
+    if (steps > 0) stage(0);
 
     // ---- outer fragments
-    bf16x8 f1[G::KSTEPS], f2[G::KSTEPS];
+    const int orow = row < nb ? row : (nb > 0 ? nb - 1 : 0);
+    bf16x8 f1[KS], f2[KS];
     float oL = INFINITY, oD = 0.f;
     if constexpr (MODE == MODE_DQ) {
-        const size_t at = ((size_t)b * N + orow) * os + (size_t)oh * DH + hi * 8;
+        const size_t at = ((size_t)b * N + orow) * opitch + (size_t)oh * DH * 2 + hi * 16;
         float d = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < G::KSTEPS; ++ks) {
-            f1[ks] = *(const bf16x8*)(base + (size_t)orow * rs + (size_t)oh * DH + ks * 16 + hi * 8);
-            f2[ks] = *(const bf16x8*)(a.dout + at + ks * 16);
-            const bf16x8 ov = *(const bf16x8*)(a.out + at + ks * 16);
+        for (int ks = 0; ks < KS; ++ks) {
+            f1[ks] = *(const bf16x8*)(base + (size_t)orow * pitch + (size_t)oh * DH * 2 + ks * 32 + hi * 16);
+            f2[ks] = *(const bf16x8*)((const unsigned char*)a.dout + at + ks * 32);
+            const bf16x8 ov = *(const bf16x8*)((const unsigned char*)a.out + at + ks * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e) d = fmaf((float)f2[ks][e], (float)ov[e], d);
         }
         oD = d + __shfl_xor(d, 32, 64);
         if (row < nb) oL = a.lse[((size_t)b * H + oh) * N + row]; else oD = 0.f;
     } else {
+        const unsigned char* kp = base + (size_t)orow * pitch + (size_t)(H + hk) * DH * 2 + hi * 16;
 #pragma unroll
-        for (int ks = 0; ks < G::KSTEPS; ++ks) {
-            f1[ks] = *(const bf16x8*)(kbase + (size_t)orow * rs + ks * 16 + hi * 8);
-            f2[ks] = *(const bf16x8*)(vbase + (size_t)orow * rs + ks * 16 + hi * 8);
+        for (int ks = 0; ks < KS; ++ks) {
+            f1[ks] = *(const bf16x8*)(kp + ks * 32);
+            f2[ks] = *(const bf16x8*)(kp + (size_t)HK * DH * 2 + ks * 32);
         }
     }
-    f32x16 acc1[G::DB], acc2[G::DB];  // DQ: acc1 = dQ^T.  DKV: acc1 = dK^T, acc2 = dV^T
+    rel_expand(a.geo, T, sl, MODE == MODE_DQ, MODE == MODE_DQ ? oh : oh * group);
+    const RelLane<MODE == MODE_DQ> rl(a.geo, sl, T, row, N - 1);
+    const TrRead<DH> tr(lane);
+    const int ro = lds0 + I::at(r, hi);
+    f32x16 acc1[DB], acc2[DB];  // DQ: acc1 = dQ^T.  DKV: acc1 = dK^T, acc2 = dV^T
 #pragma unroll
-    for (int d = 0; d < G::DB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) { acc1[d][e] = 0.f; acc2[d][e] = 0.f; }
-
-    const RelSlice sl(a.geo, blk0, blk1, MODE == MODE_DQ);  // over all keys / all queries
-    const RelLane<MODE == MODE_DQ> rl(a.geo, sl, T, row, N - 1);
-    const int nheads = MODE == MODE_DQ ? 1 : group;
     float dsum = 0.f;  // DQ: row sum of dS
-    for (int gh = 0; gh < nheads && nb > 0; ++gh) {
-        const int h = MODE == MODE_DQ ? oh : oh * group + gh;
-        __syncthreads();
-        rel_expand(a.geo, T, sl, MODE == MODE_DQ, h);
-        const bf16_t* i1 = MODE == MODE_DQ ? kbase : base + (size_t)h * DH;
-        const bf16_t* i2 = MODE == MODE_DQ ? vbase : a.dout + (size_t)b * N * os + (size_t)h * DH;
-        const size_t s2 = MODE == MODE_DQ ? rs : os;
-        const size_t sat = ((size_t)b * H + h) * N;
-        for (int ic0 = 0; ic0 < nb; ic0 += IC) {
-            int nin = nb - ic0;
-            nin = nin > IC ? IC : (nin + 31) & ~31;
-            __syncthreads();
-            for (int idx = tid; idx < nin * G::CHUNKS; idx += blockDim.x) {
-                const int rr = idx / G::CHUNKS, c = idx - rr * G::CHUNKS;
-                int gr = ic0 + rr;
-                if (gr > nb - 1) gr = nb - 1;  // pad rows re-read the last row; they are masked below
-                const bf16x8 v1 = *(const bf16x8*)(i1 + (size_t)gr * rs + c * 8);
-                const bf16x8 v2 = *(const bf16x8*)(i2 + (size_t)gr * s2 + c * 8);
-                *(bf16x8*)(R1 + (size_t)rr * G::RS + c * 16) = v1;
-                *(bf16x8*)(R2 + (size_t)rr * G::RS + c * 16) = v2;
-                *(bf16x8*)(T1 + (size_t)rr * G::TS + c * 16) = v1;
-                if constexpr (MODE == MODE_DKV) *(bf16x8*)(T2 + (size_t)rr * G::TS + c * 16) = v2;
-            }
-            for (int i = tid; i < nin; i += blockDim.x) {
-                const int gr = ic0 + i;
-                codes[i] = rel_row_code(a.geo, sl, MODE == MODE_DQ, gr);
-                if constexpr (MODE == MODE_DKV) {
-                    rowL[i] = gr < nb ? a.lse[sat + gr] : INFINITY;  // P = exp2(.. - inf) = 0 for pad queries
-                    rowD[i] = gr < nb ? a.delta[sat + gr] : 0.f;
-                }
-            }
-            __syncthreads();
-            for (int t = 0; t < nin >> 5; ++t) {
-                f32x16 s, dp;
-                rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, ic0 + t * 32);
+    int c = 0;
+    for (int step = 0; step < steps; ++step) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");  // the chunk is whole; nobody reads the other buffer (and at c = 0 T) any more
+        if (MODE == MODE_DKV && c == 0 && step > 0) {  // the next head of the group
+            rel_expand(a.geo, T, sl, false, oh * group + step / nc);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            asm volatile("s_barrier" ::: "memory");
+        }
+        if (step + 1 < steps) stage(step + 1);
+        const int img = (step & 1) * BUF, row0 = c * CR;
+        const unsigned char* const buf = smem + img;
+        f32x16 s, dp;
+        rel_tile(s, (const int*)(buf + BUF - CR * 4), rl, hi, a.geo.prefix, row0);
+        if constexpr (MODE == MODE_DQ) {
+            float nd = -oD;
+            if constexpr (DH > 64) asm volatile("" : "+v"(nd));  // (opaque: a block of 16 registers kept for it would be spilled)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) dp[e] = 0.f;
-                const unsigned char* p1 = R1 + (size_t)(t * 32 + r) * G::RS + hi * 16;
-                const unsigned char* p2 = R2 + (size_t)(t * 32 + r) * G::RS + hi * 16;
+            for (int e = 0; e < 16; ++e) dp[e] = nd;
+        } else {
 #pragma unroll
-                for (int ks = 0; ks < G::KSTEPS; ++ks) {
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(p1 + ks * 32), f1[ks], s, 0, 0, 0);
-                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(p2 + ks * 32), f2[ks], dp, 0, 0, 0);
-                }
-                if constexpr (MODE == MODE_DQ) {
-                    const int key0 = ic0 + t * 32;
-                    if (key0 + 32 > nb) {
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const f32x4 Dl = *(const f32x4*)(buf + 2 * IMG + CR * 4 + (8 * g4 + 4 * hi) * 4);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (key0 + (e & 3) + 8 * (e >> 2) + 4 * hi >= nb) s[e] = -INFINITY;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL);
-                        s[e] = p * (dp[e] - oD);  // dS^T
-                        dsum += s[e];
-                    }
-                } else {
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4) {
-                        const f32x4 L = *(const f32x4*)(rowL + t * 32 + 8 * g4 + 4 * hi);
-                        const f32x4 Dl = *(const f32x4*)(rowD + t * 32 + 8 * g4 + 4 * hi);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int e = g4 * 4 + j;
-                            const float p = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L[j]);
-                            dp[e] = p * (dp[e] - Dl[j]);  // dS
-                            s[e] = p;                     // P
-                        }
-                    }
-                }
-#pragma unroll
-                for (int sk = 0; sk < 2; ++sk) {
-                    const bf16x8 x1 = pack8b(MODE == MODE_DQ ? s : dp, sk);
-#pragma unroll
-                    for (int d = 0; d < G::DB; ++d)
-                        acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<G::TS>(T1, t * 32, sk, d, tr_key, tr_col), x1, acc1[d], 0, 0, 0);
-                    if constexpr (MODE == MODE_DKV) {
-                        const bf16x8 x2 = pack8b(s, sk);
-#pragma unroll
-                        for (int d = 0; d < G::DB; ++d)
-                            acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<G::TS>(T2, t * 32, sk, d, tr_key, tr_col), x2, acc2[d], 0, 0, 0);
-                    }
-                }
+                for (int j = 0; j < 4; ++j) dp[g4 * 4 + j] = Dl[j];
             }
         }
+        int ka = ro + img;
+        asm volatile("" : "+v"(ka));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks)), f1[ks], s, 0, 0, 0);
+            dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks) + IMG), f2[ks], dp, 0, 0, 0);
+        }
+        if (row0 + CR > nb) {
+            int lim = nb - row0 - 4 * hi;
+            asm volatile("" : "+v"(lim));
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
+        }
+        const unsigned t1 = (unsigned)(lds0 + img), t2 = t1 + IMG;
+        bf16x8 xt[DB];
+        if constexpr (MODE == MODE_DQ) {
+            tr.template read_step<0>(xt, t1);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL) * dp[e];  // dS^T
+                dsum += s[e];
+            }
+            const bf16x8 x0 = pack8b(s, 0), x1 = pack8b(s, 1);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], x0, acc1[d], 0, 0, 0);
+            tr.template read_step<1>(xt, t1);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], x1, acc1[d], 0, 0, 0);
+        } else {
+            tr.template read_step<0>(xt, t2);
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const f32x4 L = *(const f32x4*)(buf + 2 * IMG + (8 * g4 + 4 * hi) * 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = g4 * 4 + j;
+                    s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L[j]);  // P
+                    dp[e] *= s[e];                                               // dS
+                }
+            }
+            const bf16x8 p0 = pack8b(s, 0), p1 = pack8b(s, 1), d0 = pack8b(dp, 0), d1 = pack8b(dp, 1);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], p0, acc2[d], 0, 0, 0);
+            tr.template read_step<1>(xt, t2);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], p1, acc2[d], 0, 0, 0);
+            tr.template read_step<0>(xt, t1);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], d0, acc1[d], 0, 0, 0);
+            tr.template read_step<1>(xt, t1);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], d1, acc1[d], 0, 0, 0);
+        }
+        c = c + 1 == nc ? 0 : c + 1;
     }
     if constexpr (MODE == MODE_DQ) {
         dsum += __shfl_xor(dsum, 32, 64);
-        if (row < N && hi == 0) a.delta[((size_t)b * H + oh) * N + row] = oL < INFINITY ? oD + dsum : 0.f;
+        if (row < N && hi == 0) a.ndelta[((size_t)b * H + oh) * N + row] = oL < INFINITY ? -(oD + dsum) : 0.f;
     }
     // ---- store (rows behind the sample's length: zeros)
     if (row < N) {
         const bool live = row < nb;
-        bf16_t* dst = a.dqkv + ((size_t)b * N + row) * rs + (size_t)(MODE == MODE_DQ ? oh : H + oh) * DH;
+        bf16_t* dst = a.dqkv + (((size_t)b * N + row) * (H + 2 * HK) + (MODE == MODE_DQ ? oh : H + oh)) * DH;
 #pragma unroll
-        for (int d = 0; d < G::DB; ++d)
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
                 const int d0 = d * 32 + 8 * g4 + 4 * hi;
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
         if (ks1 == KS) {
             const size_t at = ((size_t)b * H + h) * N;
             nL = (a.lse + at)[qr];
-            nD = (a.delta + at)[qr];
+            nD = (a.ndelta + at)[qr];
         }
     };
     f32x16 acc[KT];
@@ -365,7 +372,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
                 f32x16 s, dp;
                 rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) dp[e] = -D;
+                for (int e = 0; e < 16; ++e) dp[e] = D;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const int off = I::at(t * 32 + r, ks * 2 + hi);
@@ -509,32 +516,12 @@ __global__ __launch_bounds__(256) void attn_rel_bucket_kernel(const RelBwdArgs a
     if (lane == 0) a.dtable[(size_t)bucket * a.H + h] = s;
 }
 
-// waves per workgroup: cover ceil(N / 32) outer tiles with the least padding, at least 4 (staging wants threads)
-int pick_waves_b(int N, int* blocks) {
-    const int n32 = ceil_div(N, 32);
-    int best_w = 4, best_cost = 1 << 30;
-    for (int w = 8; w >= 4; --w) {
-        const int cost = ceil_div(n32, w) * w;
-        if (cost < best_cost) { best_cost = cost; best_w = w; }
-    }
-    *blocks = ceil_div(n32, best_w);
-    return best_w;
-}
-
 template <int DH, int MODE>
-int launch_part(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
-    using G = BGeo<DH>;
-    constexpr int per_row = 2 * G::RS + (MODE == MODE_DKV ? 2 : 1) * G::TS + (MODE == MODE_DKV ? 8 : 0) + 4;
-    constexpr int LDS_MAX = 64 * 1024;
-    int blocks;
-    const int waves = pick_waves_b(a.N, &blocks);
-    int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
+int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t stream) {
+    const int n32 = ceil_div(a.N, 32), blocks = ceil_div(n32, 4), waves = ceil_div(n32, blocks);  // equal blocks of up to 4 waves
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
     VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
-    const int icmax = LDS_MAX / per_row / 32 * 32;
-    const int npad = (a.N + 31) / 32 * 32;
-    const int nchunks = ceil_div(npad, icmax);
-    a.IC = (ceil_div(npad, nchunks) + 31) / 32 * 32;
-    const size_t lds = (size_t)a.IC * per_row + (size_t)slice * 4;
+    const size_t lds = (size_t)2 * (2 * 32 * LdsImage<DH>::ROW + (MODE == MODE_DKV ? 512 : 256)) + (size_t)slice * 4;
     auto kern = attn_rel_bwd_kernel<DH, MODE>;
     static PerDeviceInt attr_set;
     std::atomic<int>* as = attr_set.slot();
@@ -604,7 +591,7 @@ int launch_bias_grad(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t st
 template <int DH>
 int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
     if (attention_rel_bwd_dh64_eligible(a.N, a.H, a.HK, DH)) {
-        VIT_TRY_RC(launch_attention_rel_bwd_dh64(a.geo, a.qkv, a.out, a.dout, a.lse, a.delta, a.dqkv, a.lengths, a.B, a.N, a.H, a.scale, stream));
+        VIT_TRY_RC(launch_attention_rel_bwd_dh64(a.geo, a.qkv, a.out, a.dout, a.lse, a.ndelta, a.dqkv, a.lengths, a.B, a.N, a.H, a.scale, stream));
     } else {
         VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, stream)));
         VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, stream)));
@@ -661,7 +648,7 @@ extern "C" int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, co
     a.dout = (const bf16_t*)d_out;
     a.lse = lse;
     a.dqkv = (bf16_t*)dqkv;
-    a.delta = (float*)((char*)workspace + w.delta);
+    a.ndelta = (float*)((char*)workspace + w.delta);
     a.part = (float*)((char*)workspace + w.part);
     a.doff = (float*)((char*)workspace + w.doff);
     a.dtable = d_table;

@@ -24,7 +24,7 @@ struct RelBwd64Args {
     const unsigned char* out;
     const unsigned char* dout;
     const float* lse;
-    float* delta;
+    float* ndelta;
     unsigned char* dqkv;
     const int* lengths;
     RelGeo geo;
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (hi == 0) {
             rowL[row] = oL;
             rowD[row] = -oD;
-            if (row < N) a.delta[((size_t)b * H + h) * N + row] = oD;
+            if (row < N) a.ndelta[((size_t)b * H + h) * N + row] = -oD;
         }
         // the wave's own keys for B
 #pragma unroll
@@ -373,14 +373,14 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // whole heads of 97..224 tokens, as many key as query heads
 bool attention_rel_bwd_dh64_eligible(int N, int heads, int kv_heads, int head_dim) { return head_dim == 64 && heads == kv_heads && N > 96 && N <= 224; }
 
-int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,
+int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* ndelta, void* dqkv,
                                   const int* lengths, int batch, int N, int heads, float scale, hipStream_t stream) {
     RelBwd64Args a{};
     a.qkv = (const unsigned char*)qkv;
     a.out = (const unsigned char*)out;
     a.dout = (const unsigned char*)dout;
     a.lse = lse;
-    a.delta = delta;
+    a.ndelta = ndelta;
     a.dqkv = (unsigned char*)dqkv;
     a.lengths = lengths;
     a.geo = geo;
