@@ -18,15 +18,14 @@ struct RelFwdArgs {
     float* lse;
     const int* lengths;
     RelGeo geo;
-    int N, H, HK, KC;
+    int N, H, HK;
     float scale_log2e;
 };
 
 constexpr float kDeferLog2 = 6.0f;  // the running max is left alone until a score outgrows it by more than this (base 2)
 constexpr float kFloor = -1e35f;    // a running max never falls below this: masked scores (-inf) then have probability 0
 constexpr int KCH = 32;             // keys of a staged chunk
-// waves of a workgroup: with two workgroups a CU (their LDS fits twice) as many as the head dim's registers allow, 4, 3 or 2 a SIMD
-constexpr int rel_waves(int dh) { return 4; }
+constexpr int NWAVE = 4;            // waves of a workgroup
 
 __device__ __forceinline__ bf16x8 pack8(const f32x16& p, int s) {
     bf16x8 o;
@@ -41,10 +40,12 @@ __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
 }
 
 // bf16, any head dim and length. A workgroup of up to 4 waves takes 32 queries a wave of one (sample, head); keys and values come in chunks
-// of 64 by LDS-DMA into two buffers, the next chunk under the products of this one: one barrier a chunk, and two or three workgroups a CU
-// to fill what a wave waits for (a few rows of LDS per workgroup, against whole sequences staged at once: ... ).
+// of 32 by LDS-DMA into two buffers, the next chunk under the products of this one: one barrier a chunk, and three or four workgroups a CU
+// to fill what a wave waits for. Bound by the vector instructions (softmax, bias addresses) that the matrix instructions only partly cover:
+// 4 x 1025 tokens, 16 heads of 80: 69 us, 0.31 PFLOP/s; 6 x 1777 tokens with lengths, 16 heads of 128 over 4 of keys: 153 us. With whole
+// sequences staged, one workgroup a CU, they took 75 and 195 us.
 template <int DH>
-__global__ __launch_bounds__(64 * rel_waves(DH)) __attribute__((amdgpu_waves_per_eu(DH <= 64 ? 4 : 3))) void attention_rel_bf16_kernel(const RelFwdArgs a) {
+__global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <= 64 ? 4 : 3))) void attention_rel_bf16_kernel(const RelFwdArgs a) {
     using I = LdsImage<DH>;
     constexpr int KS = DH / 16, DB = (DH + 31) / 32, IMG = KCH * I::ROW;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -177,146 +178,10 @@ __global__ __launch_bounds__(64 * rel_waves(DH)) __attribute__((amdgpu_waves_per
     }
 }
 
-// ---- fp32: the same structure on v_mfma_f32_32x32x2_f32 (exact fp32 products)
-template <int DH>
-__global__ __launch_bounds__(512) void attention_rel_f32_kernel(const RelFwdArgs a) {
-    constexpr int DB = (DH + 31) / 32;
-    constexpr int KSF = DH + 1;   // K row stride, floats (odd: conflict-free column reads)
-    constexpr int VSF = DB * 32;  // V row stride, floats
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int KC = a.KC, N = a.N, H = a.H;
-    int* codes = (int*)smem;
-    float* Kl = (float*)(codes + KC);
-    float* Vl = Kl + (size_t)KC * KSF;
-    float* T = Vl + (size_t)KC * VSF;
-
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nwaves = blockDim.x >> 6;
-    const int r = lane & 31, hi = lane >> 5;
-    const int b = blockIdx.x / H, h = blockIdx.x - b * H, hk = h / (H / a.HK);
-    const size_t rs = (size_t)(H + 2 * a.HK) * DH;
-    const float* base = (const float*)a.qkv + (size_t)b * N * rs;
-    const float* kbase = base + (size_t)(H + hk) * DH;
-    const float* vbase = kbase + (size_t)a.HK * DH;
-    const int nb = sample_length(a.lengths, b, N);
-
-    const int blk0 = blockIdx.y * nwaves * 32;
-    const int q0 = blk0 + wave * 32, q = q0 + r;
-    const int qrow = q < nb ? q : (nb > 0 ? nb - 1 : 0);
-    float qf[DH / 2];
-#pragma unroll
-    for (int t = 0; t < DH / 2; ++t) qf[t] = base[(size_t)qrow * rs + (size_t)h * DH + 2 * t + hi];
-
-    const int blk1 = blk0 + nwaves * 32 - 1;
-    const RelSlice sl(a.geo, blk0, blk1 < N ? blk1 : N - 1, true);
-    rel_expand(a.geo, T, sl, true, h);
-    const RelLane<true> rl(a.geo, sl, T, q, N - 1);
-
-    f32x16 o[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
-
-    for (int kc0 = 0; kc0 < nb; kc0 += KC) {
-        int nkeys = nb - kc0;
-        nkeys = nkeys > KC ? KC : (nkeys + 31) & ~31;
-        __syncthreads();
-        for (int idx = tid; idx < nkeys * VSF; idx += blockDim.x) {
-            const int key = idx / VSF, c = idx - key * VSF;
-            const int gk = kc0 + key;
-            float kv = 0.f, vv = 0.f;
-            if (gk < nb && c < DH) {
-                kv = kbase[(size_t)gk * rs + c];
-                vv = vbase[(size_t)gk * rs + c];
-            }
-            if (c < DH) Kl[(size_t)key * KSF + c] = kv;
-            Vl[(size_t)key * VSF + c] = vv;
-        }
-        for (int i = tid; i < nkeys; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, kc0 + i);
-        __syncthreads();
-
-        for (int t = 0; t < nkeys >> 5; ++t) {
-            const int key0 = kc0 + t * 32;
-            f32x16 s;
-            rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
-            const float* kp = Kl + (size_t)(t * 32 + r) * KSF + hi;
-#pragma unroll
-            for (int kk = 0; kk < DH / 2; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kp[2 * kk], qf[kk], s, 0, 0, 0);
-            if (key0 + 32 > nb) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (key0 + (e & 3) + 8 * (e >> 2) + 4 * hi >= nb) s[e] = -INFINITY;
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float m_new = fmaxf(m_run, mx * a.scale_log2e);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = exp2f(m_run - m_use);
-            m_run = m_new;
-            float psum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[e] = exp2f(fmaf(s[e], a.scale_log2e, -m_use));
-                psum += s[e];
-            }
-            l_run = l_run * alpha + psum;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
-            // k-step e pairs key (e & 3) + 8 (e >> 2) [lanes 0-31] with the same + 4 [lanes 32-63]: what register e holds
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float* vp = Vl + (size_t)(t * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi) * VSF + r;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vp[d * 32], s[e], o[d], 0, 0, 0);
-            }
-        }
-    }
-
-    const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-    const bool live = q < nb && (l_tot > 0.f || l_tot != l_tot);
-    const float inv = 1.0f / l_tot;
-    if (q < N) {
-        float* op = (float*)a.out + ((size_t)b * N + q) * H * DH + (size_t)h * DH;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4) {
-                const int d0 = d * 32 + 8 * g4 + 4 * hi;
-                if (d0 < DH) {
-                    f32x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = live ? o[d][g4 * 4 + e] * inv : 0.f;
-                    *(f32x4*)(op + d0) = v;
-                }
-            }
-    }
-}
-
-// waves per block: cover ceil(N / 32) query tiles with the least padding, prefer more waves
-int pick_waves(int N, int* qblocks) {
-    const int n32 = ceil_div(N, 32);
-    int best_w = 1, best_cost = 1 << 30;
-    for (int w = 8; w >= 1; --w) {
-        if (w < 4 && n32 >= 4) break;
-        const int cost = ceil_div(n32, w) * w;
-        if (cost < best_cost) { best_cost = cost; best_w = w; }
-    }
-    *qblocks = ceil_div(n32, best_w);
-    return best_w;
-}
-
 template <int DH>
 int launch_rel_bf16(RelFwdArgs a, const vit_rel_pos* pos, int batch, hipStream_t stream) {
-    const int n32 = ceil_div(a.N, 32), qblocks = ceil_div(n32, rel_waves(DH)), waves = ceil_div(n32, qblocks);  // equal blocks
+    const int n32 = ceil_div(a.N, 32), qblocks = ceil_div(n32, NWAVE), waves = ceil_div(n32, qblocks);  // equal blocks
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
-    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     const size_t lds = (size_t)4 * KCH * LdsImage<DH>::ROW + (size_t)(2 * KCH + slice) * 4;
     static PerDeviceInt attr_set;
     std::atomic<int>* as = attr_set.slot();
@@ -329,35 +194,17 @@ int launch_rel_bf16(RelFwdArgs a, const vit_rel_pos* pos, int batch, hipStream_t
     return VIT_OK;
 }
 
-template <int DH>
-int launch_rel_f32(RelFwdArgs a, const vit_rel_pos* pos, int batch, hipStream_t stream) {
-    int qblocks;
-    const int waves = pick_waves(a.N, &qblocks);
-    const int per_key = (DH + 1 + (DH + 31) / 32 * 32 + 1) * 4;
-    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
-    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
-    int KC = 80 * 1024 / per_key / 32 * 32;
-    const int npad = (a.N + 31) / 32 * 32;
-    if (KC > npad) KC = npad;
-    a.KC = KC;
-    const size_t lds = (size_t)KC * per_key + (size_t)slice * 4;
-    static PerDeviceInt attr_set;
-    std::atomic<int>* as = attr_set.slot();
-    if (!as || !as->load(std::memory_order_relaxed)) {
-        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)attention_rel_f32_kernel<DH>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        if (as) as->store(1, std::memory_order_relaxed);
-    }
-    hipLaunchKernelGGL(attention_rel_f32_kernel<DH>, dim3(batch * a.H, qblocks), dim3(waves * 64), lds, stream, a);
-    VIT_CHECK_HIP(hipGetLastError());
-    return VIT_OK;
-}
-
 }  // namespace
 
 // persistent LDS-DMA ring for head_dim 64 and whole sequences (attention_rel_dh64.hip)
 bool attention_rel_dh64_eligible(const vit_rel_pos* pos, int batch, int heads, int kv_heads);
 int launch_attention_rel_dh64(const vit_rel_pos* pos, const RelGeo& geo, const void* qkv, void* out, float* lse, int batch, int heads, int kv_heads,
                               float scale, hipStream_t stream);
+
+// fp32, and bf16 with few query rows: the waves of a workgroup share the keys (attention_rel_split.hip)
+bool attention_rel_split_eligible(const vit_rel_pos* pos, int batch, int heads, int dtype, int ncu);
+int launch_attention_rel_split(const vit_rel_pos* pos, const RelGeo& geo, const void* qkv, const int* lengths, void* out, float* lse, int batch, int heads,
+                               int kv_heads, int head_dim, float scale, int dtype, int ncu, hipStream_t stream);
 
 int rel_make_geo(const char* who, const vit_rel_pos* pos, const float* table, int heads, float scale, RelGeo* out, int* seq) {
     VIT_REQUIRE(pos && table, "%s: null argument", who);
@@ -369,7 +216,7 @@ int rel_make_geo(const char* who, const vit_rel_pos* pos, const float* table, in
     VIT_REQUIRE(pos->num_buckets > 0 && (pos->bucket_of || pos->num_buckets >= offsets + (pos->prefix ? 3 : 0)),
                 "%s: %d buckets without a map for %d offsets", who, pos->num_buckets, offsets);
     *out = RelGeo{table, pos->bucket_of, pos->prefix, pos->grid_w, pos->grid_h * pos->grid_w, (pos->grid_h - 1) * (2 * pos->grid_w - 1) + pos->grid_w - 1,
-                  offsets, pos->num_buckets, heads, 1.0f / scale};
+                  offsets, pos->num_buckets, heads, 1.0f / scale, 1.0f / (float)pos->grid_w};
     *seq = pos->prefix + pos->grid_h * pos->grid_w;
     return VIT_OK;
 }
@@ -395,10 +242,16 @@ extern "C" int vit_attention_rel_fwd(const vit_rel_pos* pos, const void* qkv, co
     a.HK = kv_heads;
     a.scale_log2e = scale * LOG2E;
     VIT_REQUIRE((int64_t)a.N * (heads + 2 * kv_heads) * head_dim * (dtype == VIT_BF16 ? 2 : 4) < (1LL << 31), "vit_attention_rel_fwd: one sample's qkv rows exceed 2 GiB");
-    if (dtype == VIT_BF16 && head_dim == 64 && !lengths && attention_rel_dh64_eligible(pos, batch, heads, kv_heads))
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, 128);
+    VIT_REQUIRE(slice <= kRelSliceCap, "vit_attention_rel_fwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
+    int ncu = 0;
+    VIT_TRY_RC(vit_cu_count(&ncu));
+    if (attention_rel_split_eligible(pos, batch, heads, dtype, ncu))
+        return launch_attention_rel_split(pos, a.geo, qkv, lengths, out, lse, batch, heads, kv_heads, head_dim, scale, dtype, ncu, (hipStream_t)stream);
+    if (head_dim == 64 && !lengths && attention_rel_dh64_eligible(pos, batch, heads, kv_heads))
         return launch_attention_rel_dh64(pos, a.geo, qkv, out, lse, batch, heads, kv_heads, scale, (hipStream_t)stream);
 #define REL_CASE(DHV) \
-    case DHV: return dtype == VIT_BF16 ? launch_rel_bf16<DHV>(a, pos, batch, (hipStream_t)stream) : launch_rel_f32<DHV>(a, pos, batch, (hipStream_t)stream);
+    case DHV: return launch_rel_bf16<DHV>(a, pos, batch, (hipStream_t)stream);
     switch (head_dim) {
         REL_CASE(16) REL_CASE(32) REL_CASE(48) REL_CASE(64) REL_CASE(80) REL_CASE(96) REL_CASE(112) REL_CASE(128)
     }

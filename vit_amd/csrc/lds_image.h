@@ -1,6 +1,6 @@
 // Rows of one head (DH bf16 values each) as an LDS image filled by LDS-DMA: 16-byte chunks, a wave instruction writes 64 of them
 // lane-linear. Conflict-free for ds_read_b128 of one chunk column over 16 consecutive rows:
-//  * 8 or 16 chunks a row (head_dim 64, 128): unpadded, chunk c of row r sits at position c ^ swizzle(r). For 8 chunks the swizzle is
+//  * 8, 16 or 32 chunks a row (bf16 head_dim 64, 128; fp32 rows of twice the width): unpadded, chunk c of row r sits at position c ^ swizzle(r). For 8 chunks the swizzle is
 //    the bit reversal of (r >> 1) & 7, with which ds_read_b64_tr_b16 of 8 consecutive rows x 64 bytes is conflict-free too (rows r and
 //    r + 2 differ in the position's highest bit), so one image serves row reads and transposed reads.
 //  * other widths: one chunk of padding a row (an odd number of chunks); the lanes on the padding re-read the row's last chunk.
@@ -10,13 +10,13 @@
 template <int DH>
 struct LdsImage {
     static constexpr int CH = DH / 8;                       // 16-byte chunks of a row
-    static constexpr bool SWZ = CH == 8 || CH == 16;
+    static constexpr bool SWZ = CH == 8 || CH == 16 || CH == 32;
     static constexpr int PCH = SWZ ? CH : CH + 1;           // chunks a row takes in LDS
     static constexpr int ROW = PCH * 16;                    // bytes
     static constexpr int RPI = 64 / PCH;                    // rows a wave instruction fills
     static __device__ __forceinline__ int swizzle(int row) {
         if constexpr (CH == 8) return ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3);
-        else if constexpr (CH == 16) return row & 15;
+        else if constexpr (SWZ) return row & 15;
         else return 0;
     }
     // byte offset of chunk c of a row

@@ -14,7 +14,7 @@ struct RelGeo {
     const float* table;    // [num_buckets, heads]
     const int* bucket_of;  // [offsets + 3] or null: the index itself
     int prefix, gw, grid, center, offsets, num_buckets, heads;
-    float inv_scale;
+    float inv_scale, inv_gw;
 };
 
 constexpr float kRelMasked = -1e30f;  // a table entry below this masks its offset (a mask written as a type's lowest value)
@@ -23,7 +23,8 @@ __device__ __forceinline__ int rel_code(const RelGeo& g, int token) {
     int p = token - g.prefix;
     p = p < 0 ? 0 : p;
     p = p > g.grid - 1 ? g.grid - 1 : p;
-    return p + (p / g.gw) * (g.gw - 1);
+    // row of the cell: (p + 1/2) / gw is at least 1 / (2 gw) from a whole number, 16 times what rounding adds for p < 2^14 and more
+    return p + (int)(((float)p + 0.5f) * g.inv_gw) * (g.gw - 1);
 }
 // bias of an offset index in units of the raw product (divided by the softmax scale): the start value of the product's
 // accumulator, so that adding it costs nothing
