@@ -61,23 +61,20 @@ __global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <
     const int pitch = (H + 2 * a.HK) * DH * 2;
     const unsigned char* base = (const unsigned char*)a.qkv + (size_t)b * N * pitch;
     const int nb = __builtin_amdgcn_readfirstlane(sample_length(a.lengths, b, N));
-    const int blk0 = (gridDim.y - 1 - blockIdx.y) * nw * 32, blk1 = blk0 + nw * 32 - 1;  // (last blocks first: only long samples have them)
+    // with lengths the last blocks first (only long samples have them), else last (the sequence may end inside one)
+    const int blk0 = (a.lengths ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * nw * 32, blk1 = blk0 + nw * 32 - 1;
     const int q0 = blk0 + wave * 32, q = q0 + r;
     const int nc = blk0 < nb ? (nb + KCH - 1) / KCH : 0;  // (a block of rows behind the sample only stores zeros)
 
     const __amdgpu_buffer_rsrc_t kr = head_resource<DH>(base + (size_t)(H + hk) * DH * 2, N, pitch);
     const __amdgpu_buffer_rsrc_t vr = head_resource<DH>(base + (size_t)(H + a.HK + hk) * DH * 2, N, pitch);
     const RelSlice sl(a.geo, blk0, blk1 < N ? blk1 : N - 1, true);
+    const LdsFill<DH> fill(lane);
     auto stage = [&](int c) {
         unsigned char* const dst = smem + (c & 1) * 2 * IMG;
-        // whole tiles up to the sample's last key (rows behind it re-read that key: what is masked is still finite)
-        const int need = nb - c * KCH < KCH ? (nb - c * KCH + 31) & ~31 : KCH;
-        int ln = lane;
-        asm volatile("" : "+v"(ln));  // (opaque: the lane offsets are made here, not kept in registers over the products)
-        for (int i = wave * I::RPI; i < need; i += nw * I::RPI) {
-            I::dma(kr, dst, i, KCH, c * KCH, nb - 1, pitch, ln);
-            I::dma(vr, dst + IMG, i, KCH, c * KCH, nb - 1, pitch, ln);
-        }
+        // (rows behind the sample re-read its last key: what is masked is still finite)
+        fill.chunk(kr, dst, KCH, wave, nw, c * KCH, nb - 1, pitch);
+        fill.chunk(vr, dst + IMG, KCH, wave, nw, c * KCH, nb - 1, pitch);
         for (int i = tid; i < KCH; i += blockDim.x) codes[(c & 1) * KCH + i] = rel_row_code(a.geo, sl, true, c * KCH + i);
     };
     if (nc > 0) stage(0);
@@ -103,17 +100,15 @@ __global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <
         asm volatile("s_barrier" ::: "memory");  // the chunk is whole; nobody reads the other buffer any more
         if (c + 1 < nc) stage(c + 1);
         const int img = (c & 1) * 2 * IMG;
-#pragma unroll 1
-        for (int t = 0; t < KCH / 32; ++t) {
-            const int key0 = c * KCH + t * 32;
-            if (key0 >= nb) break;
+        {
+            const int key0 = c * KCH;
             f32x16 s;
-            rel_tile(s, codes + (c & 1) * KCH + t * 32, rl, hi, a.geo.prefix, key0);
-            int ka = ro + img + t * 32 * I::ROW;
+            rel_tile(s, codes + (c & 1) * KCH, rl, hi, a.geo.prefix, key0);
+            int ka = ro + img;
             asm volatile("" : "+v"(ka));
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks)), qf[ks], s, 0, 0, 0);
-            const unsigned vimg = lds0 + (unsigned)(img + IMG + t * 32 * I::ROW);
+            const unsigned vimg = lds0 + (unsigned)(img + IMG);
             bf16x8 vt[2][DB];
             if constexpr (DB == 4) tr.template read_step<0>(vt[0], vimg);  // (32 registers at once would cost a wave a SIMD)
             else tr.read(vt, vimg);

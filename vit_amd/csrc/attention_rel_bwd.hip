@@ -81,7 +81,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
     const int b = blockIdx.x / OH, oh = blockIdx.x - b * OH, group = H / HK;
     const int pitch = (H + 2 * HK) * DH * 2, opitch = H * DH * 2;
     const int nb = __builtin_amdgcn_readfirstlane(sample_length(a.lengths, b, N));
-    const int blk0 = (gridDim.y - 1 - blockIdx.y) * nw * 32;  // (last blocks first: only long samples have them)
+    // with lengths the last blocks first (only long samples have them), else last (the sequence may end inside one)
+    const int blk0 = (a.lengths ? gridDim.y - 1 - blockIdx.y : blockIdx.y) * nw * 32;
     const int blk1 = min(blk0 + nw * 32, N) - 1;
     const int o0 = blk0 + wave * 32, row = o0 + r;
     const unsigned char* base = (const unsigned char*)a.qkv + (size_t)b * N * pitch;
@@ -91,19 +92,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
     const int nc = blk0 < nb ? (nb + CR - 1) / CR : 0, steps = nc * nheads;
     const RelSlice sl(a.geo, blk0, blk1, MODE == MODE_DQ);  // over all keys / all queries
 
-    auto stage = [&](int step) {
-        const int gh = step / nc, c = step - gh * nc, h = MODE == MODE_DQ ? oh : oh * group + gh, row0 = c * CR;
+    const LdsFill<DH> fill(lane);
+    auto stage = [&](int step, int h, int c) {
+        const int row0 = c * CR;
         unsigned char* const dst = smem + (step & 1) * BUF;
         // rows behind the sample re-read its last one: what is masked is still finite
         const __amdgpu_buffer_rsrc_t r1 = head_resource<DH>(base + (size_t)(MODE == MODE_DQ ? H + hk : h) * DH * 2, N, pitch);
         const __amdgpu_buffer_rsrc_t r2 = MODE == MODE_DQ ? head_resource<DH>(base + (size_t)(H + HK + hk) * DH * 2, N, pitch)
                                                           : head_resource<DH>(gbase + (size_t)h * DH * 2, N, opitch);
         int ln = lane;
-        asm volatile("" : "+v"(ln));  // (opaque: the lane offsets are made here, not kept in registers over the products)
-        for (int i = wave * I::RPI; i < CR; i += nw * I::RPI) {
-            I::dma(r1, dst, i, CR, row0, nb - 1, pitch, ln);
-            I::dma(r2, dst + IMG, i, CR, row0, nb - 1, MODE == MODE_DQ ? pitch : opitch, ln);
-        }
+        asm volatile("" : "+v"(ln));  // (opaque: what follows is made here, not kept in registers over the products)
+        fill.chunk(r1, dst, CR, wave, nw, row0, nb - 1, pitch);
+        fill.chunk(r2, dst + IMG, CR, wave, nw, row0, nb - 1, MODE == MODE_DQ ? pitch : opitch);
         if constexpr (MODE == MODE_DKV) {
             if (wave == 0) {  // the queries' lse and -delta
                 const size_t at = ((size_t)b * H + h) * N;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
         }
         if (ln < CR && wave == nw - 1) *(int*)(dst + BUF - CR * 4 + ln * 4) = rel_row_code(a.geo, sl, MODE == MODE_DQ, row0 + ln);
     };
-    if (steps > 0) stage(0);
+    if (steps > 0) stage(0, MODE == MODE_DQ ? oh : oh * group, 0);
 
     // ---- outer fragments
     const int orow = row < nb ? row : (nb > 0 ? nb - 1 : 0);
@@ -156,16 +156,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
 #pragma unroll
         for (int e = 0; e < 16; ++e) { acc1[d][e] = 0.f; acc2[d][e] = 0.f; }
     float dsum = 0.f;  // DQ: row sum of dS
-    int c = 0;
+    int c = 0, head = MODE == MODE_DQ ? oh : oh * group;
     for (int step = 0; step < steps; ++step) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");  // the chunk is whole; nobody reads the other buffer (and at c = 0 T) any more
         if (MODE == MODE_DKV && c == 0 && step > 0) {  // the next head of the group
-            rel_expand(a.geo, T, sl, false, oh * group + step / nc);
+            rel_expand(a.geo, T, sl, false, head);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             asm volatile("s_barrier" ::: "memory");
         }
-        if (step + 1 < steps) stage(step + 1);
+        if (step + 1 < steps) stage(step + 1, c + 1 == nc ? head + 1 : head, c + 1 == nc ? 0 : c + 1);
         const int img = (step & 1) * BUF, row0 = c * CR;
         const unsigned char* const buf = smem + img;
         f32x16 s, dp;
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], d1, acc1[d], 0, 0, 0);
         }
-        c = c + 1 == nc ? 0 : c + 1;
+        if (++c == nc) { c = 0; ++head; }
     }
     if constexpr (MODE == MODE_DQ) {
         dsum += __shfl_xor(dsum, 32, 64);
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
     using I = LdsImage<DH>;
     constexpr int KS = DH / 16, ROWS = KT * 32, IMG = ROWS * I::ROW;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    // [2][K image, V image], the keys' codes, the expansion; after the samples: [waves * 32][33] sums, then the folded vector
+    // [2][K image, V image], the keys' codes, the expansion; after the samples what the fold needs
     int* const codes = (int*)(smem + 4 * IMG);
     float* const T = (float*)(codes + ROWS);
     const int tid = threadIdx.x, lane = tid & 63;
@@ -287,11 +287,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
     const int pitch = (H + 2 * HK) * DH * 2, opitch = H * DH * 2;
     const int b0 = (int)((int64_t)B * blockIdx.z / a.splits), b1 = (int)((int64_t)B * (blockIdx.z + 1) / a.splits);
     const int blk1 = blk0 + nw * 32 < N ? blk0 + nw * 32 - 1 : N - 1;
-    const RelSlice sl(a.geo, blk0, blk1, true);
-    rel_expand(a.geo, T, sl, true, h);
-    for (int i = tid; i < ROWS; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, k0 + i);
-    const RelLane<true> rl(a.geo, sl, T, q, N - 1);
-    __syncthreads();
 
     auto next_sample = [&](int b) {  // the first from b on that has a pair in this block
         while (b < b1) {
@@ -352,6 +347,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
         load_rows(b, nb, 0, KS);
         stage(b, nb, 0, 0, pieces);
     }
+    const RelSlice sl(a.geo, blk0, blk1, true);  // (under the first sample's loads)
+    rel_expand(a.geo, T, sl, true, h);
+    for (int i = tid; i < ROWS; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, k0 + i);
+    const RelLane<true> rl(a.geo, sl, T, q, N - 1);
     while (b < b1) {
         const int bn = next_sample(b + 1), nnb = bn < b1 ? sample_length(a.lengths, bn, N) : 0;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -395,71 +394,87 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
         buf ^= 1;
     }
 
-    // ---- fold, one strip of 32 keys at a time: thread = diagonal i - j of the strip; vector place v = its offset from the block's lowest
-    const int nq32 = nw * 32, nd = nq32 + 31;
-    float* const S = (float*)smem;         // [nq32][33]
-    float* const V = S + nq32 * 33;        // [2 (nq32 + ROWS - 1)]
-    float* const P3 = V + 2 * (nq32 + ROWS - 1);  // [8][3]
+    // ---- fold. Each wave its own 32 x 32 tiles through LDS: lane (r, hi) adds the pairs (i, j = (i + r) mod 32), i = 16 hi .. 16 hi + 15,
+    // which lie on two diagonals, i - j = -r and, past the tile's edge, 32 - r; the first of tile t is the second of tile t + 1.
+    float* const S = (float*)smem + wave * (32 * 33);  // [32][33]
+    float* const V = (float*)smem + nw * (32 * 33);    // [nw][KT + 1][class][32]: offset q0 - k0 + 32 - 32 slot - r
+    float* const P3 = V + nw * (KT + 1) * 64;          // [nw][3]
     const int prefix = a.geo.prefix, gw = a.geo.gw;
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f;
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f, c0 = 0.f, c1 = 0.f;
+    auto modw = [&](int v) {
+        v %= gw;
+        return v < 0 ? v + gw : v;
+    };
+    auto emit = [&](int slot, float v0, float v1) {
+        v0 += __shfl_xor(v0, 32, 64);
+        v1 += __shfl_xor(v1, 32, 64);
+        V[((wave * (KT + 1) + slot) * 2 + hi) * 32 + r] = hi ? v1 : v0;
+    };
     __syncthreads();
-    for (int i = tid; i < 2 * (nq32 + ROWS - 1); i += blockDim.x) V[i] = 0.f;
-    for (int t = 0; t < KT && k0 + t * 32 < N; ++t) {
-        __syncthreads();
+    const int x0 = modw(q0 + 16 * hi - prefix);  // column of the lane's first query (a prefix token's is not used)
+    int dx = modw(q0 - k0 - r), dx2 = modw(q0 - k0 + 32 - r);
 #pragma unroll
-        for (int u = 0; u < KT; ++u) {
-            if (u != t) continue;  // (uniform; the accumulators need constant indices)
+    for (int t = 0; t < KT; ++t) {
+        __builtin_amdgcn_wave_barrier();  // (the last tile's reads come first)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) S[(wave * 32 + r) * 33 + (e & 3) + 8 * (e >> 2) + 4 * hi] = acc[u][e];
-        }
-        __syncthreads();
-        for (int g = tid; g < nd; g += blockDim.x) {
-            const int o = blk0 - (k0 + t * 32) + g - 31;  // query token - key token
-            int dx = o % gw;
-            if (dx < 0) dx += gw;
-            const int p = blk0 + g - 31 - prefix;  // place of the query at j = 0
-            int x = p % gw;
-            if (x < 0) x += gw;
-            // the diagonal's pairs: rows 0 .. nq32 - 1 of the strip, both tokens on the grid and in the sequence
-            int j0 = 31 - g > -p ? 31 - g : -p, j1 = nq32 + 31 - g;
-            if (prefix - (k0 + t * 32) > j0) j0 = prefix - (k0 + t * 32);
-            if (N - (k0 + t * 32) < j1) j1 = N - (k0 + t * 32);
-            if (N - (blk0 + g - 31) < j1) j1 = N - (blk0 + g - 31);
-            float a0 = 0.f, a1 = 0.f;
-#pragma unroll 8
-            for (int j = 0; j < 32; ++j) {
-                const bool in = j >= j0 && j < j1;
-                const float v = S[in ? (g - 31) * 33 + j * 34 : 0];
-                a0 += in && x >= dx ? v : 0.f;
-                a1 += in && x < dx ? v : 0.f;
+        for (int e = 0; e < 16; ++e) S[r * 33 + (e & 3) + 8 * (e >> 2) + 4 * hi] = acc[t][e];
+        __builtin_amdgcn_wave_barrier();
+        float a10 = 0.f, a11 = 0.f, a20 = 0.f, a21 = 0.f;
+        if (q0 < prefix || k0 + t * 32 < prefix) {  // a tile with prefix tokens: those pairs in three sums of their own
+            const int lq = prefix - q0, lk = prefix - (k0 + t * 32);
+            int x = x0;
+            for (int n = 0; n < 16; ++n) {
+                const int i = 16 * hi + n, j = (i + r) & 31;
+                const float v = S[i * 33 + j];
+                const bool grid = i >= lq && j >= lk, wrap = i + r >= 32, low = x >= (wrap ? dx2 : dx);
+                a10 += grid && !wrap && low ? v : 0.f;
+                a11 += grid && !wrap && !low ? v : 0.f;
+                a20 += grid && wrap && low ? v : 0.f;
+                a21 += grid && wrap && !low ? v : 0.f;
+                s0 += i < lq && j >= lk ? v : 0.f;
+                s1 += i >= lq && j < lk ? v : 0.f;
+                s2 += i < lq && j < lk ? v : 0.f;
                 x = x + 1 == gw ? 0 : x + 1;
             }
-            const int v = g + 32 * (KT - 1 - t);
-            V[2 * v] += a0;
-            V[2 * v + 1] += a1;
-        }
-        if (prefix > 0 && (tq == 0 || tk == 0) && tid < nq32) {
-            const int tokq = blk0 + tid;
-            for (int j = 0; j < 32; ++j) {
-                const int key = k0 + t * 32 + j;
-                if (tokq >= N || key >= N) continue;
-                const float v = S[tid * 33 + j];
-                if (tokq < prefix) {
-                    if (key < prefix) s2 += v; else s0 += v;
-                } else if (key < prefix) {
-                    s1 += v;
-                }
+        } else {
+            int x = x0;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                const int i = 16 * hi + n;
+                const float v = S[i * 33 + ((i + r) & 31)];
+                const bool wrap = i + r >= 32, low = x >= (wrap ? dx2 : dx);
+                const float v0 = low ? v : 0.f, v1 = low ? 0.f : v;
+                a10 += wrap ? 0.f : v0;
+                a11 += wrap ? 0.f : v1;
+                a20 += wrap ? v0 : 0.f;
+                a21 += wrap ? v1 : 0.f;
+                x = x + 1 == gw ? 0 : x + 1;
             }
         }
+        emit(t, c0 + a20, c1 + a21);
+        c0 = a10, c1 = a11;
+        dx2 = dx;
+        dx = modw(dx - 32);
     }
-    s0 = wave_sum(s0);
-    s1 = wave_sum(s1);
-    s2 = wave_sum(s2);
+    emit(KT, c0, c1);
+    if (prefix > 0) {
+        s0 = wave_sum(s0);
+        s1 = wave_sum(s1);
+        s2 = wave_sum(s2);
+    }
     if (lane == 0) { P3[wave * 3] = s0; P3[wave * 3 + 1] = s1; P3[wave * 3 + 2] = s2; }
     __syncthreads();
-    const int fold = 2 * (nq32 + ROWS - 1);
+    const int fold = 2 * (nw * 32 + ROWS - 1);  // place v: offset blk0 - k0 + v - (ROWS - 1)
     float* dst = a.part + ((((size_t)blockIdx.z * H + h) * a.tq + tq) * a.tk + tk) * a.fp;
-    for (int i = tid; i < fold; i += blockDim.x) dst[i] = V[i];
+    for (int i = tid; i < fold; i += blockDim.x) {
+        const int o = (i >> 1) - (ROWS - 1), m = (o + 32 * KT + 31) / 32 - KT;  // o = 32 m - r
+        float v = 0.f;
+        for (int w = 0; w < nw; ++w) {
+            const int slot = w + 1 - m;
+            if (slot >= 0 && slot <= KT) v += V[((w * (KT + 1) + slot) * 2 + (i & 1)) * 32 + 32 * m - o];
+        }
+        dst[i] = v;
+    }
     if (tid < 3) {
         float v = 0.f;
         for (int w = 0; w < nw; ++w) v += P3[w * 3 + tid];
@@ -467,32 +482,42 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
     }
 }
 
-// ---- per offset: the blocks' folded sums in a fixed order. One wave per (offset index, head): lanes over (split, query block)
-__global__ __launch_bounds__(256) void attn_rel_offset_kernel(const RelBwdArgs a, float* dst, int stride_h, int stride_o) {
-    const int lane = threadIdx.x & 63;
-    const int idx = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y;
-    const int offsets = a.geo.offsets;
-    if (idx >= offsets + (a.geo.prefix ? 3 : 0)) return;  // wave-uniform
+// ---- per offset: the blocks' folded sums in a fixed order. A lane has an offset index (neighbours read neighbours) of one head, a
+// workgroup's waves share its (split, query block) pairs
+constexpr int kOffsetWaves = 16;
+__global__ __launch_bounds__(64 * kOffsetWaves) void attn_rel_offset_kernel(const RelBwdArgs a, float* dst, int stride_h, int stride_o) {
+    __shared__ float sums[kOffsetWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int idx = blockIdx.x * 64 + lane, h = blockIdx.y;
+    const int offsets = a.geo.offsets, all = offsets + (a.geo.prefix ? 3 : 0);
     const int gw = a.geo.gw, rows = 2 * gw - 1;
     const int dyi = idx / rows, dx = idx - dyi * rows - (gw - 1), dy = dyi - (a.geo.center / rows);
     const int o = dy * gw + dx, cls = dx < 0 ? 1 : 0;
     const int bq = a.bq, bk = a.bk, fold = bq + bk - 1;  // queries, keys of a block, diagonals
     float s = 0.f;
-    for (int i = lane; i < a.splits * a.tq; i += 64) {
-        const int sp = i / a.tq, tq = i - sp * a.tq;
-        const float* p = a.part + (((size_t)sp * a.H + h) * a.tq + tq) * a.tk * a.fp;
-        if (idx >= offsets) {
-            for (int tk = 0; tk < a.tk; ++tk)
-                if (tq == 0 || tk == 0) s += p[(size_t)tk * a.fp + 2 * fold + idx - offsets];
-        } else {
+    if (idx < offsets) {
+        for (int i = wave; i < a.splits * a.tq; i += kOffsetWaves) {
+            const int sp = i / a.tq, tq = i - sp * a.tq;
+            const float* p = a.part + (((size_t)sp * a.H + h) * a.tq + tq) * a.tk * a.fp;
             // key blocks that hold a key i - o of the block's queries
             const int j0 = tq * bq - o, j1 = j0 + bq - 1;  // keys of its first and last query
             const int t0 = j0 > 0 ? j0 / bk : 0, t1 = j1 < 0 ? -1 : j1 / bk;
             for (int tk = t0; tk <= t1 && tk < a.tk; ++tk) s += p[(size_t)tk * a.fp + 2 * (o - (tq * bq - tk * bk) + bk - 1) + cls];
         }
+    } else if (idx < all) {  // the prefix classes: only the first blocks have any
+        for (int i = wave; i < a.splits * a.tq; i += kOffsetWaves) {
+            const int sp = i / a.tq, tq = i - sp * a.tq;
+            const float* p = a.part + (((size_t)sp * a.H + h) * a.tq + tq) * a.tk * a.fp;
+            for (int tk = 0; tk < (tq == 0 ? a.tk : 1); ++tk) s += p[(size_t)tk * a.fp + 2 * fold + idx - offsets];
+        }
     }
-    s = wave_sum(s);
-    if (lane == 0) dst[(size_t)h * stride_h + (size_t)idx * stride_o] = s;
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave > 0 || idx >= all) return;
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kOffsetWaves; ++w) s += sums[w][lane];
+    dst[(size_t)h * stride_h + (size_t)idx * stride_o] = s;
 }
 // ---- per bucket: its offsets' sums in the map's order
 __global__ __launch_bounds__(256) void attn_rel_bucket_kernel(const RelBwdArgs a) {
@@ -573,7 +598,7 @@ int launch_bias_grad(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t st
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, a.bq);
     VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     size_t lds = bias_lds(DH, KT, slice);
-    const size_t fold = ((size_t)a.bq * 33 + 2 * (a.bq + KT * 32 - 1) + 24) * 4;
+    const size_t fold = (size_t)nw * (32 * 33 + (KT + 1) * 64 + 3) * 4;
     if (lds < fold) lds = fold;
     VIT_REQUIRE(lds <= 160 * 1024, "attention_rel_bwd: head_dim %d with %d bias entries does not fit the LDS", DH, slice);
     auto kern = attn_rel_bias_grad_kernel<DH, KT>;
@@ -597,13 +622,13 @@ int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
         VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, stream)));
     }
     if (!a.dtable) return VIT_OK;
-    if (a.bk == 7 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 64 ? 7 : 4)>(a, pos, stream)));
+    if (a.bk == 7 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 64 ? 7 : DH <= 112 ? 4 : 2)>(a, pos, stream)));
     else if (a.bk == 4 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 112 ? 4 : 2)>(a, pos, stream)));
     else VIT_TRY_RC((launch_bias_grad<DH, 2>(a, pos, stream)));
     const int total = a.geo.offsets + (a.geo.prefix ? 3 : 0);
     // without a map, and with nothing in the table behind the offsets, the offset sums are the table's gradient
     const bool direct = !a.geo.bucket_of && a.geo.num_buckets == total;
-    hipLaunchKernelGGL(attn_rel_offset_kernel, dim3(ceil_div(total, 4), a.H), dim3(256), 0, stream, a, direct ? a.dtable : a.doff,
+    hipLaunchKernelGGL(attn_rel_offset_kernel, dim3(ceil_div(total, 64), a.H), dim3(64 * kOffsetWaves), 0, stream, a, direct ? a.dtable : a.doff,
                        direct ? 1 : total, direct ? a.H : 1);
     VIT_CHECK_HIP(hipGetLastError());
     if (!direct) {

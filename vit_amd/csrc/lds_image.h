@@ -35,6 +35,38 @@ struct LdsImage {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, LDS_PTR(dst + r0 * ROW), 16, src * pitch + c * 16, 0, 0, 0);
     }
 };
+// The same for whole chunks in a loop: what a lane adds to a piece's address is made once; a chunk that ends before the sample does
+// needs no more per instruction than a scalar offset.
+template <int DH>
+struct LdsFill {
+    using I = LdsImage<DH>;
+    int rr, c16;  // the lane's row of a piece, its chunk's byte in the row
+    __device__ __forceinline__ LdsFill(int lane) {
+        const int pos = lane - lane / I::PCH * I::PCH;
+        rr = lane / I::PCH;
+        c16 = (I::SWZ ? pos ^ I::swizzle(rr) : pos < I::CH ? pos : I::CH - 1) << 4;
+    }
+    // pieces first, first + step .. of an image of `rows` rows
+    __device__ __forceinline__ void chunk(__amdgpu_buffer_rsrc_t rsrc, unsigned char* dst, int rows, int first, int step, int src_row0, int src_last,
+                                          int pitch) const {
+        if (src_row0 + rows - 1 <= src_last) {
+            const int lane_off = rr * pitch + (I::SWZ ? 0 : c16);
+            for (int i = first * I::RPI; i < rows; i += step * I::RPI) {
+                const int off = I::SWZ ? lane_off + (c16 ^ (I::swizzle(i) << 4)) : lane_off;  // (a piece's row and a lane's have no bit in common)
+                if (rr < (rows - i < I::RPI ? rows - i : I::RPI))
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, LDS_PTR(dst + i * I::ROW), 16, off, (src_row0 + i) * pitch, 0, 0);
+            }
+        } else {
+            for (int i = first * I::RPI; i < rows; i += step * I::RPI) {
+                const int off = I::SWZ ? c16 ^ (I::swizzle(i) << 4) : c16;
+                int src = src_row0 + i + rr;
+                src = src < src_last ? src : src_last;
+                if (rr < (rows - i < I::RPI ? rows - i : I::RPI))
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, LDS_PTR(dst + i * I::ROW), 16, src * pitch + off, 0, 0, 0);
+            }
+        }
+    }
+};
 // 16 bytes at an LDS address
 __device__ __forceinline__ bf16x8 lds_chunk(int addr) { return *(__attribute__((address_space(3))) const bf16x8*)(uintptr_t)addr; }
 // buffer resource over `rows` rows of one head, `pitch` bytes apart

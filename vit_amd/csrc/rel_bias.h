@@ -28,11 +28,28 @@ __device__ __forceinline__ int rel_code(const RelGeo& g, int token) {
 }
 // bias of an offset index in units of the raw product (divided by the softmax scale): the start value of the product's
 // accumulator, so that adding it costs nothing
+template <int U>
+__device__ __forceinline__ void rel_entries(const RelGeo& g, const int (&index)[U], int head, float (&v)[U]) {  // the loads of all U together
+    int b[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) b[j] = index[j];
+    if (g.bucket_of) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) b[j] = g.bucket_of[index[j]];
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int c = b[j] < 0 ? 0 : b[j] < g.num_buckets ? b[j] : g.num_buckets - 1;
+        v[j] = g.table[(size_t)c * g.heads + head];
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) v[j] = b[j] < 0 || b[j] >= g.num_buckets ? 0.f : v[j] < kRelMasked ? -INFINITY : v[j] * g.inv_scale;
+}
 __device__ __forceinline__ float rel_entry(const RelGeo& g, int index, int head) {
-    const int b = g.bucket_of ? g.bucket_of[index] : index;
-    if (b < 0 || b >= g.num_buckets) return 0.f;
-    const float v = g.table[(size_t)b * g.heads + head];
-    return v < kRelMasked ? -INFINITY : v * g.inv_scale;
+    const int at[1] = {index};
+    float v[1];
+    rel_entries<1>(g, at, head, v);
+    return v[0];
 }
 // The slice of offsets that the queries first .. last of a block reach over all keys (query), or the keys first .. last over all
 // queries: entries lo .. lo + n - 1. Behind it in LDS, with a prefix: span + 1 copies of the entry of a prefix token on the other side,
@@ -53,7 +70,19 @@ struct RelSlice {
 __device__ __forceinline__ void rel_expand(const RelGeo& g, float* T, const RelSlice& s, bool query, int head) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // (opaque: nothing of this is worth a register in the loops around it)
-    for (int i = tid; i < s.n; i += blockDim.x) T[i] = rel_entry(g, s.lo + i, head);
+    for (int i = tid; i < s.n; i += 4 * blockDim.x) {  // four entries' loads under way at once
+        int at[4];
+        float v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            at[j] = i + j * (int)blockDim.x;
+            at[j] = s.lo + (at[j] < s.n ? at[j] : s.n - 1);
+        }
+        rel_entries<4>(g, at, head, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j * (int)blockDim.x < s.n) T[i + j * (int)blockDim.x] = v[j];
+    }
     if (g.prefix) {
         const float other = rel_entry(g, g.offsets + (query ? 1 : 0), head);
         for (int i = tid; i <= s.span; i += blockDim.x) T[s.n + i] = other;
