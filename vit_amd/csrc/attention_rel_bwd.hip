@@ -61,6 +61,90 @@ __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
     return n < 0 ? 0 : n > N ? N : n;
 }
 
+// Buffers of a chunk of 32 inner rows: two images, (lse, -delta), codes; a multiple of 256 (LdsImage::step)
+constexpr int CR = 32;
+template <int DH, int MODE>
+constexpr int chunk_bytes() { return 2 * CR * LdsImage<DH>::ROW + (MODE == MODE_DKV ? 512 : 256); }
+
+// One chunk's products, for 32 outer rows on the lane: `buf` its buffer (at LDS address img; ro: of the lane's first row piece)
+template <int DH, int MODE>
+__device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsigned char* buf, int img, int ro, const TrRead<DH>& tr,
+                                               const RelLane<MODE == MODE_DQ>& rl, const bf16x8 (&f1)[DH / 16], const bf16x8 (&f2)[DH / 16], float oL,
+                                               float oD, f32x16 (&acc1)[(DH + 31) / 32], f32x16 (&acc2)[(DH + 31) / 32], float& dsum, int row0, int nb,
+                                               int hi) {
+    using I = LdsImage<DH>;
+    constexpr int KS = DH / 16, DB = (DH + 31) / 32, IMG = CR * I::ROW, BUF = chunk_bytes<DH, MODE>();
+    f32x16 s, dp;
+    rel_tile(s, (const int*)(buf + BUF - CR * 4), rl, hi, a.geo.prefix, row0);
+    if constexpr (MODE == MODE_DQ) {
+        float nd = -oD;
+        if constexpr (DH > 64) asm volatile("" : "+v"(nd));  // (opaque: a block of 16 registers kept for it would be spilled)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dp[e] = nd;
+    } else {
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+            const f32x4 Dl = *(const f32x4*)(buf + 2 * IMG + CR * 4 + (8 * g4 + 4 * hi) * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dp[g4 * 4 + j] = Dl[j];
+        }
+    }
+    int ka = ro;
+    asm volatile("" : "+v"(ka));
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks)), f1[ks], s, 0, 0, 0);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks) + IMG), f2[ks], dp, 0, 0, 0);
+    }
+    if (row0 + CR > nb) {
+        int lim = nb - row0 - 4 * hi;
+        asm volatile("" : "+v"(lim));
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
+    }
+    const unsigned t1 = (unsigned)img, t2 = t1 + IMG;
+    bf16x8 xt[DB];
+    if constexpr (MODE == MODE_DQ) {
+        tr.template read_step<0>(xt, t1);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL) * dp[e];  // dS^T
+            dsum += s[e];
+        }
+        const bf16x8 x0 = pack8b(s, 0), x1 = pack8b(s, 1);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], x0, acc1[d], 0, 0, 0);
+        tr.template read_step<1>(xt, t1);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], x1, acc1[d], 0, 0, 0);
+    } else {
+        tr.template read_step<0>(xt, t2);
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+            const f32x4 L = *(const f32x4*)(buf + 2 * IMG + (8 * g4 + 4 * hi) * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = g4 * 4 + j;
+                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L[j]);  // P
+                dp[e] *= s[e];                                               // dS
+            }
+        }
+        const bf16x8 p0 = pack8b(s, 0), p1 = pack8b(s, 1), d0 = pack8b(dp, 0), d1 = pack8b(dp, 1);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], p0, acc2[d], 0, 0, 0);
+        tr.template read_step<1>(xt, t2);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], p1, acc2[d], 0, 0, 0);
+        tr.template read_step<0>(xt, t1);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], d0, acc1[d], 0, 0, 0);
+        tr.template read_step<1>(xt, t1);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], d1, acc1[d], 0, 0, 0);
+    }
+}
+
 // what the registers allow without a spill (a spilled register's reload waits for all loads under way)
 constexpr int bwd_waves_per_simd(int dh, int mode) { return mode == MODE_DQ ? (dh <= 96 ? 3 : 2) : dh <= 64 ? 3 : dh <= 96 ? 2 : 1; }
 // A workgroup of up to 4 waves takes 32 outer rows a wave of one (sample, head); the inner rows come in chunks of 32 by LDS-DMA into two
@@ -68,8 +152,7 @@ constexpr int bwd_waves_per_simd(int dh, int mode) { return mode == MODE_DQ ? (d
 template <int DH, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_per_simd(DH, MODE)))) void attn_rel_bwd_kernel(const RelBwdArgs a) {
     using I = LdsImage<DH>;
-    constexpr int KS = DH / 16, DB = (DH + 31) / 32, CR = 32, IMG = CR * I::ROW;
-    constexpr int BUF = 2 * IMG + (MODE == MODE_DKV ? 512 : 256);  // two images, (lse, -delta), codes; a multiple of 256 (LdsImage::step)
+    constexpr int KS = DH / 16, DB = (DH + 31) / 32, IMG = CR * I::ROW, BUF = chunk_bytes<DH, MODE>();
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     float* const T = (float*)(smem + 2 * BUF);
     const int lds0 = (int)(uintptr_t)LDS_PTR(smem);
@@ -168,75 +251,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
         if (step + 1 < steps) stage(step + 1, c + 1 == nc ? head + 1 : head, c + 1 == nc ? 0 : c + 1);
         const int img = (step & 1) * BUF, row0 = c * CR;
         const unsigned char* const buf = smem + img;
-        f32x16 s, dp;
-        rel_tile(s, (const int*)(buf + BUF - CR * 4), rl, hi, a.geo.prefix, row0);
-        if constexpr (MODE == MODE_DQ) {
-            float nd = -oD;
-            if constexpr (DH > 64) asm volatile("" : "+v"(nd));  // (opaque: a block of 16 registers kept for it would be spilled)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dp[e] = nd;
-        } else {
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4) {
-                const f32x4 Dl = *(const f32x4*)(buf + 2 * IMG + CR * 4 + (8 * g4 + 4 * hi) * 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) dp[g4 * 4 + j] = Dl[j];
-            }
-        }
-        int ka = ro + img;
-        asm volatile("" : "+v"(ka));
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks)), f1[ks], s, 0, 0, 0);
-            dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_chunk(I::step(ka, ks) + IMG), f2[ks], dp, 0, 0, 0);
-        }
-        if (row0 + CR > nb) {
-            int lim = nb - row0 - 4 * hi;
-            asm volatile("" : "+v"(lim));
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
-        }
-        const unsigned t1 = (unsigned)(lds0 + img), t2 = t1 + IMG;
-        bf16x8 xt[DB];
-        if constexpr (MODE == MODE_DQ) {
-            tr.template read_step<0>(xt, t1);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL) * dp[e];  // dS^T
-                dsum += s[e];
-            }
-            const bf16x8 x0 = pack8b(s, 0), x1 = pack8b(s, 1);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], x0, acc1[d], 0, 0, 0);
-            tr.template read_step<1>(xt, t1);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], x1, acc1[d], 0, 0, 0);
-        } else {
-            tr.template read_step<0>(xt, t2);
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4) {
-                const f32x4 L = *(const f32x4*)(buf + 2 * IMG + (8 * g4 + 4 * hi) * 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int e = g4 * 4 + j;
-                    s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L[j]);  // P
-                    dp[e] *= s[e];                                               // dS
-                }
-            }
-            const bf16x8 p0 = pack8b(s, 0), p1 = pack8b(s, 1), d0 = pack8b(dp, 0), d1 = pack8b(dp, 1);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], p0, acc2[d], 0, 0, 0);
-            tr.template read_step<1>(xt, t2);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc2[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], p1, acc2[d], 0, 0, 0);
-            tr.template read_step<0>(xt, t1);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], d0, acc1[d], 0, 0, 0);
-            tr.template read_step<1>(xt, t1);
-#pragma unroll
-            for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], d1, acc1[d], 0, 0, 0);
-        }
+        chunk_products<DH, MODE>(a, buf, lds0 + img, ro + img, tr, rl, f1, f2, oL, oD, acc1, acc2, dsum, row0, nb, hi);
         if (++c == nc) { c = 0; ++head; }
     }
     if constexpr (MODE == MODE_DQ) {
@@ -541,12 +556,204 @@ __global__ __launch_bounds__(256) void attn_rel_bucket_kernel(const RelBwdArgs a
     if (lane == 0) a.dtable[(size_t)bucket * a.H + h] = s;
 }
 
+// ---- the same for few outer rows: a workgroup has 32 of them, its waves share the inner chunks (wave w takes w, w + waves, .., each through
+// its own buffer, no barrier between), and their sums are added through LDS.
+constexpr int split_waves_most(int dh, int mode) { return mode == MODE_DKV && dh > 96 ? 4 : 8; }  // (two waves a SIMD have 256 registers each)
 template <int DH, int MODE>
-int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t stream) {
-    const int n32 = ceil_div(a.N, 32), blocks = ceil_div(n32, 4), waves = ceil_div(n32, blocks);  // equal blocks of up to 4 waves
+__global__ __launch_bounds__(64 * split_waves_most(DH, MODE)) void attn_rel_bwd_split_kernel(const RelBwdArgs a, int tile0) {
+    using I = LdsImage<DH>;
+    constexpr int KS = DH / 16, DB = (DH + 31) / 32, IMG = CR * I::ROW, BUF = chunk_bytes<DH, MODE>(), OUT = MODE == MODE_DQ ? 3 : 2;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x >> 6;
+    const int r = lane & 31, hi = lane >> 5;
+    unsigned char* const rows = smem + (size_t)nw * BUF;  // images of the outer rows: DQ Q, dO, O;  DKV K, V
+    float* const sums = (float*)(rows + OUT * IMG);       // [nw][32]: DQ the waves' row sums of dS
+    float* const T = sums + nw * 32;
+    unsigned char* const buf = smem + (size_t)wave * BUF;
+    const int img = (int)(uintptr_t)LDS_PTR(buf);
+    const int N = a.N, H = a.H, HK = a.HK;
+    const int OH = MODE == MODE_DQ ? H : HK;  // outer heads
+    const int b = blockIdx.x / OH, oh = blockIdx.x - b * OH, group = H / HK;
+    const int pitch = (H + 2 * HK) * DH * 2, opitch = H * DH * 2;
+    const int nb = __builtin_amdgcn_readfirstlane(sample_length(a.lengths, b, N));
+    const int o0 = (tile0 + blockIdx.y) * 32, row = o0 + r;
+    const unsigned char* base = (const unsigned char*)a.qkv + (size_t)b * N * pitch;
+    const unsigned char* gbase = (const unsigned char*)a.dout + (size_t)b * N * opitch;
+    const int hk = MODE == MODE_DQ ? oh / group : oh, head0 = MODE == MODE_DQ ? oh : oh * group;
+    const int nheads = MODE == MODE_DQ ? 1 : group;
+    const int nc = o0 < nb ? (nb + CR - 1) / CR : 0;
+    const RelSlice sl(a.geo, o0, min(o0 + 31, N - 1), MODE == MODE_DQ);
+    const LdsFill<DH> fill(lane);
+    auto stage = [&](int h, int c) {  // the wave's next chunk
+        const int row0 = c * CR;
+        // rows behind the sample re-read its last one: what is masked is still finite
+        const __amdgpu_buffer_rsrc_t r1 = head_resource<DH>(base + (size_t)(MODE == MODE_DQ ? H + hk : h) * DH * 2, N, pitch);
+        const __amdgpu_buffer_rsrc_t r2 = MODE == MODE_DQ ? head_resource<DH>(base + (size_t)(H + HK + hk) * DH * 2, N, pitch)
+                                                          : head_resource<DH>(gbase + (size_t)h * DH * 2, N, opitch);
+        fill.chunk(r1, buf, CR, 0, 1, row0, nb - 1, pitch);
+        fill.chunk(r2, buf + IMG, CR, 0, 1, row0, nb - 1, MODE == MODE_DQ ? pitch : opitch);
+        if constexpr (MODE == MODE_DKV) {
+            const size_t at = ((size_t)b * H + h) * N;
+            int q = row0 + lane;
+            q = q < nb ? q : nb - 1;
+            const __amdgpu_buffer_rsrc_t rl_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.lse + at), 0, (unsigned)N * 4, 0x00020000);
+            const __amdgpu_buffer_rsrc_t rd_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.ndelta + at), 0, (unsigned)N * 4, 0x00020000);
+            if (lane < CR) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rl_, LDS_PTR(buf + 2 * IMG), 4, q * 4, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rd_, LDS_PTR(buf + 2 * IMG + CR * 4), 4, q * 4, 0, 0, 0);
+            }
+        }
+        if (lane < CR) *(int*)(buf + BUF - CR * 4 + lane * 4) = rel_row_code(a.geo, sl, MODE == MODE_DQ, row0 + lane);
+    };
+    if (nc > 0) {
+        if constexpr (MODE == MODE_DQ) {
+            fill.chunk(head_resource<DH>(base + (size_t)oh * DH * 2, N, pitch), rows, CR, wave, nw, o0, nb - 1, pitch);
+            fill.chunk(head_resource<DH>(gbase + (size_t)oh * DH * 2, N, opitch), rows + IMG, CR, wave, nw, o0, nb - 1, opitch);
+            const unsigned char* ob = (const unsigned char*)a.out + (size_t)b * N * opitch + (size_t)oh * DH * 2;
+            fill.chunk(head_resource<DH>(ob, N, opitch), rows + 2 * IMG, CR, wave, nw, o0, nb - 1, opitch);
+        } else {
+            fill.chunk(head_resource<DH>(base + (size_t)(H + hk) * DH * 2, N, pitch), rows, CR, wave, nw, o0, nb - 1, pitch);
+            fill.chunk(head_resource<DH>(base + (size_t)(H + HK + hk) * DH * 2, N, pitch), rows + IMG, CR, wave, nw, o0, nb - 1, pitch);
+        }
+        if (wave < nc) stage(head0, wave);
+    }
+    float oL = INFINITY, oD = 0.f;
+    if (MODE == MODE_DQ && row < nb) oL = a.lse[((size_t)b * H + oh) * N + row];
+    rel_expand(a.geo, T, sl, MODE == MODE_DQ, head0);
+    const RelLane<MODE == MODE_DQ> rl(a.geo, sl, T, row, N - 1);
+    const TrRead<DH> tr(lane);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // the outer rows, T
+    bf16x8 f1[KS], f2[KS];
+    if (nc > 0) {
+        float d = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            f1[ks] = *(const bf16x8*)(rows + I::at(r, 2 * ks + hi));
+            f2[ks] = *(const bf16x8*)(rows + IMG + I::at(r, 2 * ks + hi));
+            if constexpr (MODE == MODE_DQ) {
+                const bf16x8 ov = *(const bf16x8*)(rows + 2 * IMG + I::at(r, 2 * ks + hi));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d = fmaf((float)f2[ks][e], (float)ov[e], d);
+            }
+        }
+        if (MODE == MODE_DQ && row < nb) oD = d;
+        if constexpr (MODE == MODE_DQ) oD += __shfl_xor(oD, 32, 64);
+    }
+    f32x16 acc1[DB], acc2[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { acc1[d][e] = 0.f; acc2[d][e] = 0.f; }
+    float dsum = 0.f;
+    for (int g = 0; g < nheads; ++g) {
+        if (g > 0) {  // the next head of the group
+            __syncthreads();
+            rel_expand(a.geo, T, sl, false, head0 + g);
+            __syncthreads();
+        }
+        for (int c = wave; c < nc; c += nw) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            chunk_products<DH, MODE>(a, buf, img, img + I::at(r, hi), tr, rl, f1, f2, oL, oD, acc1, acc2, dsum, c * CR, nb, hi);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the chunk's reads are over)
+            if (c + nw < nc) stage(head0 + g, c + nw);
+            else if (g + 1 < nheads) stage(head0 + g + 1, wave);
+        }
+    }
+    // ---- the waves' sums
+    if constexpr (MODE == MODE_DQ) {
+        dsum += __shfl_xor(dsum, 32, 64);
+        if (hi == 0) sums[wave * 32 + r] = dsum;
+    }
+    float* const part = (float*)smem;  // [nw] of BUF bytes: [DH][32]
+    auto add = [&](f32x16 (&acc)[DB], bf16_t* dst, int rowel, float scale) {
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int dd = d * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi;
+                if (dd < DH) part[(size_t)wave * (BUF / 4) + dd * 32 + r] = acc[d][e];
+            }
+        __syncthreads();
+        for (int i = tid; i < 32 * (DH / 8); i += blockDim.x) {
+            const int q = i & 31, d0 = (i >> 5) * 8;
+            if (o0 + q >= N) continue;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+            for (int w = 0; w < nw; ++w)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += part[(size_t)w * (BUF / 4) + (d0 + e) * 32 + q];
+            bf16x8 o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = (bf16_t)(o0 + q < nb ? v[e] * scale : 0.f);  // (rows behind the sample's length: zeros)
+            *(bf16x8*)(dst + (size_t)(o0 + q) * rowel + d0) = o;
+        }
+    };
+    const int rowel = (H + 2 * HK) * DH;
+    bf16_t* dst = a.dqkv + (size_t)b * N * rowel + (size_t)(MODE == MODE_DQ ? oh : H + oh) * DH;
+    add(acc1, dst, rowel, a.scale);
+    if constexpr (MODE == MODE_DKV) add(acc2, dst + (size_t)HK * DH, rowel, 1.f);
+    if constexpr (MODE == MODE_DQ) {
+        if (wave == 0 && hi == 0 && row < N) {
+            float t = 0.f;
+            for (int w = 0; w < nw; ++w) t += sums[w * 32 + r];
+            a.ndelta[((size_t)b * H + oh) * N + row] = oL < INFINITY ? -(oD + t) : 0.f;
+        }
+    }
+}
+
+// few enough tiles of 32 rows that the waves of a workgroup share one
+// Whole calls in us, this / the kernels that share inner chunks, 12 heads of 64 (tiles a CU in brackets): 577 tokens, 1 sample [0.9] 42 / 79,
+// 2 [1.8] 65 / 86, 4 [3.6] 107 / 95; against one pass (attention_rel_bwd_dh64.hip) 197 tokens, 1 sample [0.3] 44 / 51, 4 [1.3] 56 / 52;
+// 8 heads over 4 of 128, 512 tokens, 1 sample [0.5, 0.25 for dK, dV] 52 / 130
+bool attn_rel_few_rows(int64_t tiles, int ncu, bool one_pass) { return 2 * tiles <= (one_pass ? 2 : 5) * (int64_t)ncu; }
+
+template <int DH, int MODE>
+int launch_split(const RelBwdArgs& a, const vit_rel_pos* pos, int tile0, int tiles, hipStream_t stream) {
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, 32);
+    const int n32 = ceil_div(a.N, 32);
+    int waves = n32 < split_waves_most(DH, MODE) ? n32 : split_waves_most(DH, MODE);
+    auto need = [&](int w) {
+        return (size_t)w * (chunk_bytes<DH, MODE>() + 128) + (MODE == MODE_DQ ? 3 : 2) * CR * LdsImage<DH>::ROW + (size_t)slice * 4;
+    };
+    while (waves > 1 && need(waves) > 160 * 1024) --waves;
+    auto kern = attn_rel_bwd_split_kernel<DH, MODE>;
+    static PerDeviceInt attr_set;
+    std::atomic<int>* as = attr_set.slot();
+    if (!as || !as->load(std::memory_order_relaxed)) {
+        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (as) as->store(1, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(kern, dim3(a.B * (MODE == MODE_DQ ? a.H : a.HK), tiles), dim3(waves * 64), need(waves), stream, a, tile0);
+    VIT_CHECK_HIP(hipGetLastError());
+    return VIT_OK;
+}
+
+template <int DH, int MODE>
+int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, int ncu, hipStream_t stream) {
+    const int n32 = ceil_div(a.N, 32), items = a.B * (MODE == MODE_DQ ? a.H : a.HK);
+    int blocks = ceil_div(n32, 4), waves = ceil_div(n32, blocks), tail = 0;  // equal blocks of up to 4 waves
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
     VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
-    const size_t lds = (size_t)2 * (2 * 32 * LdsImage<DH>::ROW + (MODE == MODE_DKV ? 512 : 256)) + (size_t)slice * 4;
+    if (attn_rel_few_rows((int64_t)items * n32, ncu, false)) return launch_split<DH, MODE>(a, pos, 0, n32, stream);
+    size_t lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)slice * 4;
+    if (!a.lengths && n32 > 4 && n32 % 4 && (int64_t)items * (n32 % 4) <= ncu) {
+        // Tiles behind the last whole block of 4 that would start a round of workgroups of their own: by the waves of workgroups instead
+        // (4 x 1025 tokens, 16 heads of 80, dK and dV: 131 us with the 33rd tile as a ninth block, 84 + 19 so)
+        const int big = rel_slice_max(pos->grid_h, pos->grid_w, 128);
+        const size_t big_lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)big * 4;
+        const int by_lds = (int)(160 * 1024 / big_lds), by_regs = bwd_waves_per_simd(DH, MODE);
+        const int64_t slots = (int64_t)ncu * (by_lds < by_regs ? by_lds : by_regs), full = (int64_t)items * (n32 / 4);
+        if (big <= kRelSliceCap && (full + items + slots - 1) / slots > (full + slots - 1) / slots) {
+            waves = 4;
+            blocks = n32 / 4;
+            tail = n32 % 4;
+            lds = big_lds;
+        }
+    }
     auto kern = attn_rel_bwd_kernel<DH, MODE>;
     static PerDeviceInt attr_set;
     std::atomic<int>* as = attr_set.slot();
@@ -554,9 +761,9 @@ int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t stream)
         VIT_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (as) as->store(1, std::memory_order_relaxed);
     }
-    hipLaunchKernelGGL(kern, dim3(a.B * (MODE == MODE_DQ ? a.H : a.HK), blocks), dim3(waves * 64), lds, stream, a);
+    hipLaunchKernelGGL(kern, dim3(items, blocks), dim3(waves * 64), lds, stream, a);
     VIT_CHECK_HIP(hipGetLastError());
-    return VIT_OK;
+    return tail ? launch_split<DH, MODE>(a, pos, blocks * 4, tail, stream) : VIT_OK;
 }
 
 struct Workspace {
@@ -579,6 +786,16 @@ int plan_workspace(const vit_rel_pos* pos, int batch, int heads, int head_dim, W
     w->bq = ceil_div(n32, w->tq) * 32;
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, w->bq);
     w->bk = (head_dim <= 64 && n32 > 4 && n32 <= 7 ? 7 : head_dim <= 112 && bias_lds(head_dim, 4, slice) <= 160 * 1024 ? 4 : 2) * 32;
+    // Few samples: blocks of 1, 2 or 4 key tiles, the smallest that gives each CU at most one block and three (block, sample) pairs. us at
+    // 7 / 4 / 2 / 1 tiles, 12 heads of 64 x 197 tokens: 1 sample 26 / 18 / 13 / 10, 8: 26 / 18 / 16 / 16, 64: 49 / 44 / 48 / 65; 577 tokens
+    // (more blocks than CUs at 2 tiles): 1 sample - / 18 / 22 / 25, 64: - / 268 / 347 / 454
+    for (int kt = 1; kt * 32 < w->bk; kt *= 2) {
+        const int64_t blocks = (int64_t)heads * w->tq * ceil_div(n32, kt);
+        if (blocks <= ncu && blocks * batch <= 3 * (int64_t)ncu) {
+            w->bk = kt * 32;
+            break;
+        }
+    }
     w->tk = ceil_div(N, w->bk);
     w->fp = 2 * (w->bq + w->bk - 1) + 4;
     // enough sample ranges to give every CU a workgroup, whole samples each
@@ -615,14 +832,17 @@ int launch_bias_grad(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t st
 
 template <int DH>
 int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
-    if (attention_rel_bwd_dh64_eligible(a.N, a.H, a.HK, DH)) {
+    int ncu = 0;
+    VIT_TRY_RC(vit_cu_count(&ncu));
+    if (attention_rel_bwd_dh64_eligible(a.N, a.H, a.HK, DH) && !attn_rel_few_rows((int64_t)a.B * a.H * ceil_div(a.N, 32), ncu, true)) {
         VIT_TRY_RC(launch_attention_rel_bwd_dh64(a.geo, a.qkv, a.out, a.dout, a.lse, a.ndelta, a.dqkv, a.lengths, a.B, a.N, a.H, a.scale, stream));
     } else {
-        VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, stream)));
-        VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, stream)));
+        VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, ncu, stream)));
+        VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, ncu, stream)));
     }
     if (!a.dtable) return VIT_OK;
-    if (a.bk == 7 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 64 ? 7 : DH <= 112 ? 4 : 2)>(a, pos, stream)));
+    if (a.bk == 32) VIT_TRY_RC((launch_bias_grad<DH, 1>(a, pos, stream)));
+    else if (a.bk == 7 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 64 ? 7 : DH <= 112 ? 4 : 2)>(a, pos, stream)));
     else if (a.bk == 4 * 32) VIT_TRY_RC((launch_bias_grad<DH, (DH <= 112 ? 4 : 2)>(a, pos, stream)));
     else VIT_TRY_RC((launch_bias_grad<DH, 2>(a, pos, stream)));
     const int total = a.geo.offsets + (a.geo.prefix ? 3 : 0);
