@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int U = 4;  // heads a lane has in flight
+constexpr int U = 5;  // heads a lane has in flight
 
 struct QkArgs {
     const void* x;    // packed projection output
@@ -124,6 +124,15 @@ struct Turn {
     }
 };
 
+// a head's 8 weights of a lane's chunk (any 4-byte alignment); lanes past the head take the first chunk's, which meet zeros
+__device__ __forceinline__ void load8(float (&w)[8], const float* p, int chunk, bool on) {
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    const f32x4u* v = (const f32x4u*)(p + (on ? chunk * 8 : 0));
+    const f32x4u lo = v[0], hi = v[1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { w[e] = lo[e]; w[4 + e] = hi[e]; }
+}
+
 // mean, 1 / deviation and the normalised values of a head; lanes past the head hold zeros and stay out of the sums
 template <int GL, bool LAYER>
 __device__ __forceinline__ float normalise(float (&x)[8], bool on, float inv_dh, float eps) {
@@ -148,59 +157,65 @@ template <typename T, int GL, bool LAYER, bool IL>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkArgs a) {
     constexpr int HS = 64 / GL;  // heads side by side in a wave
     const int lane = threadIdx.x & 63, slot = lane / GL, chunk = lane % GL;
-    const int wave = blockIdx.x * 4 + (threadIdx.x >> 6), waves = gridDim.x * 4;
+    const int wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = gridDim.x * 4;
     const bool on = chunk * 8 < a.dh;
     const int nh = a.heads + a.kv_heads;
+    const int all = a.out != a.x ? nh + a.kv_heads : nh;  // out of place the values pass through, as heads behind the keys
     const size_t row = (size_t)(nh + a.kv_heads) * a.dh;
     const float inv_dh = 1.0f / (float)a.dh;
+    Raw8<T> raw[U];
+    auto load_heads = [&](int tok, int h0) {
+        const T* xr = (const T*)a.x + (size_t)tok * row + chunk * 8;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + u * HS + slot;
+            if (on && h < all) raw[u].load(xr + (size_t)h * a.dh); else raw[u].zero();
+        }
+    };
+    if (wave < a.tokens) load_heads(wave, 0);  // (ahead of the weights: a small call is one token a wave)
     float w[2][8], b[2][8];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) {
+        load8(w[k], a.w[k], chunk, on);
+        if constexpr (LAYER) {
+            if (a.b[k]) {
+                load8(b[k], a.b[k], chunk, on);
+            } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            w[k][e] = on ? a.w[k][chunk * 8 + e] : 0.f;
-            b[k][e] = (LAYER && on && a.b[k]) ? a.b[k][chunk * 8 + e] : 0.f;
+                for (int e = 0; e < 8; ++e) b[k][e] = 0.f;
+            }
         }
+    }
     Turn<GL, IL> turn;
     turn.place(lane, chunk, a.rot_dim);
     for (int tok = wave; tok < a.tokens; tok += waves) {
-        const T* xr = (const T*)a.x + (size_t)tok * row + chunk * 8;
         T* yr = (T*)a.out + (size_t)tok * row + chunk * 8;
         turn.load(a, tok, chunk);
-        for (int h0 = 0; h0 < nh; h0 += HS * U) {
-            Raw8<T> raw[U];
+        for (int h0 = 0; h0 < all; h0 += HS * U) {
+            if (h0 > 0) load_heads(tok, h0);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int h = h0 + u * HS + slot;
-                if (on && h < nh) raw[u].load(xr + (size_t)h * a.dh); else raw[u].zero();
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (h0 + u * HS >= nh) break;
-                const int h = h0 + u * HS + slot;
+                if (h0 + u * HS >= all) break;
+                int h = h0 + u * HS + slot;
+                asm volatile("" : "+v"(h));  // (opaque: the weights chosen for each of the heads would be kept in registers)
                 const bool isk = h >= a.heads;
                 float y[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[e] = raw[u].get(e);
-                normalise<GL, LAYER>(y, on, inv_dh, a.eps);
+                if (h0 + u * HS < nh) {  // (uniform: some head of the group is a query or a key)
+                    normalise<GL, LAYER>(y, on, inv_dh, a.eps);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float we = isk ? w[1][e] : w[0][e];
-                    if constexpr (LAYER) y[e] = fmaf(y[e], we, isk ? b[1][e] : b[0][e]); else y[e] *= we;
+                    for (int e = 0; e < 8; ++e) {
+                        const float we = isk ? w[1][e] : w[0][e];
+                        if constexpr (LAYER) y[e] = fmaf(y[e], we, isk ? b[1][e] : b[0][e]); else y[e] *= we;
+                    }
+                    turn.template apply<1>(y);
                 }
-                turn.template apply<1>(y);
                 if (on && h < nh) Raw8<T>::store(yr + (size_t)h * a.dh, y);
+                else if (on && h < all) *(Raw8<T>*)(yr + (size_t)h * a.dh) = raw[u];
             }
         }
-        if (a.out != a.x) {  // the values pass through
-            const int nv = a.kv_heads * a.dh / 8;
-            const size_t v0 = (size_t)tok * row + (size_t)nh * a.dh;
-            for (int i = lane; i < nv; i += 64) {
-                Raw8<T> v;
-                v.load((const T*)a.x + v0 + i * 8);
-                *(Raw8<T>*)((T*)a.out + v0 + i * 8) = v;
-            }
-        }
+        if (tok + waves < a.tokens) load_heads(tok + waves, 0);
     }
 }
 
@@ -210,44 +225,48 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(const QkArgs a) {
     constexpr int NS = LAYER ? 4 : 2;  // sums kept: dw of q, k (and db of q, k)
     __shared__ float part[4][4][128];
     const int lane = threadIdx.x & 63, slot = lane / GL, chunk = lane % GL;
-    const int wib = threadIdx.x >> 6;
+    const int wib = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = blockIdx.x * 4 + wib, waves = gridDim.x * 4;
     const bool on = chunk * 8 < a.dh;
     const int nh = a.heads + a.kv_heads;
     const size_t row = (size_t)(nh + a.kv_heads) * a.dh;
     const float inv_dh = 1.0f / (float)a.dh;
-    float w[2][8], sum[NS][8];
+    Raw8<T> rx[UB], rg[UB];
+    auto load_heads = [&](int tok, int h0) {
+        const T* xr = (const T*)a.x + (size_t)tok * row + chunk * 8;
+        const T* gr = (const T*)a.g + (size_t)tok * row + chunk * 8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        w[0][e] = on ? a.w[0][chunk * 8 + e] : 0.f;
-        w[1][e] = on ? a.w[1][chunk * 8 + e] : 0.f;
+        for (int u = 0; u < UB; ++u) {
+            const int h = h0 + u * HS + slot;
+            if (on && h < nh) {
+                rx[u].load(xr + (size_t)h * a.dh);
+                rg[u].load(gr + (size_t)h * a.dh);
+            } else {
+                rx[u].zero();
+                rg[u].zero();
+            }
+        }
+    };
+    if (wave < a.tokens) load_heads(wave, 0);  // (ahead of the weights: a small call is one token a wave)
+    float w[2][8], sum[NS][8];
+    load8(w[0], a.w[0], chunk, on);
+    load8(w[1], a.w[1], chunk, on);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
         for (int k = 0; k < NS; ++k) sum[k][e] = 0.f;
-    }
     Turn<GL, IL> turn;
     turn.place(lane, chunk, a.rot_dim);
     for (int tok = wave; tok < a.tokens; tok += waves) {
-        const T* xr = (const T*)a.x + (size_t)tok * row + chunk * 8;
-        const T* gr = (const T*)a.g + (size_t)tok * row + chunk * 8;
         T* dr = (T*)a.out + (size_t)tok * row + chunk * 8;
         turn.load(a, tok, chunk);
         for (int h0 = 0; h0 < nh; h0 += HS * UB) {
-            Raw8<T> rx[UB], rg[UB];
-#pragma unroll
-            for (int u = 0; u < UB; ++u) {
-                const int h = h0 + u * HS + slot;
-                if (on && h < nh) {
-                    rx[u].load(xr + (size_t)h * a.dh);
-                    rg[u].load(gr + (size_t)h * a.dh);
-                } else {
-                    rx[u].zero();
-                    rg[u].zero();
-                }
-            }
+            if (h0 > 0) load_heads(tok, h0);
 #pragma unroll
             for (int u = 0; u < UB; ++u) {
                 if (h0 + u * HS >= nh) break;
-                const int h = h0 + u * HS + slot;
+                int h = h0 + u * HS + slot;
+                asm volatile("" : "+v"(h));  // (opaque: the weights chosen for each of the heads would be kept in registers)
                 const bool isk = h >= a.heads;
                 const float mk = isk ? 1.f : 0.f, mq = 1.f - mk;
                 float x[8], t[8];
@@ -285,6 +304,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(const QkArgs a) {
                 *(Raw8<T>*)((T*)a.out + v0 + i * 8) = v;
             }
         }
+        if (tok + waves < a.tokens) load_heads(tok + waves, 0);
     }
     // heads side by side, then the block's four waves; fixed order
 #pragma unroll
