@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkArgs a) {
 }
 
 template <typename T, int GL, bool LAYER, bool IL>
-__global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(const QkArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void qk_norm_rope_bwd_kernel(const QkArgs a) {
     constexpr int HS = 64 / GL, UB = 2;
     constexpr int NS = LAYER ? 4 : 2;  // sums kept: dw of q, k (and db of q, k)
     __shared__ float part[4][4][128];
