@@ -342,11 +342,15 @@ def _vec(t, name: str, n: int, ref: torch.Tensor, what: str):
         return None
     if t.shape != (n,):
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}, expected ({n},)")
-    return _near(t, name, ref).float().contiguous()
+    return _single(_near(t, name, ref))
+
+
+def _single(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _near(t: torch.Tensor, name: str, ref: torch.Tensor) -> torch.Tensor:
-    if t.device != ref.device:
+    if t.get_device() != ref.get_device():
         raise ValueError(f"{name} is on {t.device}, qkv on {ref.device}")
     return t
 
@@ -372,7 +376,7 @@ def _qk_norm_args(qkv, num_heads, num_kv_heads, eps, rope, positions, interleave
     if rope is not None:
         if rope.dim() != 3 or rope.shape[2] != 2 or rope.shape[0] == 0:
             raise ValueError(f"{what}: rope must be [positions, rot_dim / 2, 2], got {tuple(rope.shape)}")
-        rope = _near(rope, "rope", qkv).float().contiguous()
+        rope = _single(_near(rope, "rope", qkv))
         rope_len, rot_dim = rope.shape[0], 2 * rope.shape[1]
     if positions is not None:
         if rope is None:
@@ -459,7 +463,7 @@ def _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, what
         raise ValueError(f"{what}: qkv has {n} tokens, the buckets are for {buckets.seq}")
     if table.shape != (buckets.num_buckets, num_heads):
         raise ValueError(f"{what}: table has shape {tuple(table.shape)}, expected ({buckets.num_buckets}, {num_heads})")
-    table = _near(table, "table", qkv).float().contiguous()
+    table = _single(_near(table, "table", qkv))
     if buckets.bucket_of is not None:
         _near(buckets.bucket_of, "buckets", qkv)
     if lengths is not None:
