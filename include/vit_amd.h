@@ -280,7 +280,7 @@ typedef struct vit_rel_pos {
  * lengths: int32 [batch] device, tokens in use of each sample (keys behind are not read, rows behind give zeros), or NULL.
  * lse (VIT_BF16 only, may be NULL): [batch, heads, seq], the base-2 log-sum-exp that the backward takes (+inf where there
  * is no key). A grid too large for the LDS expansion of a query block's offsets (16384 entries:
- * beyond 88 x 88, or 1 x 16128 tokens) is refused. */
+ * beyond 89 x 89, or 1 x 16127 tokens; the backward with d_table, whose blocks are larger, beyond 88 x 88 or 1 x 15871) is refused. */
 int vit_attention_rel_fwd(const vit_rel_pos* pos, const void* qkv, const float* table, const int32_t* lengths, void* out,
                           float* lse, int batch, int heads, int kv_heads, int head_dim, float scale, int dtype,
                           void* stream);

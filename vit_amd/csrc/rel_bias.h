@@ -114,19 +114,16 @@ struct RelLane {
         any = __any(lp);
     }
 };
-typedef int i32x16 __attribute__((ext_vector_type(16)));
-// the rows' codes into registers, and with them the start values (two steps: a pipelined loop puts other work between them)
-__device__ __forceinline__ void rel_codes(i32x16& c, const int* codes, int hi) {
+template <bool QLANE>
+__device__ __forceinline__ void rel_tile(f32x16& s, const int* codes, const RelLane<QLANE>& l, int hi, int prefix, int row0) {
     typedef int i32x4 __attribute__((ext_vector_type(4)));
+    int c[16];
 #pragma unroll
     for (int g4 = 0; g4 < 4; ++g4) {
         const i32x4 v = *(const i32x4*)(codes + 8 * g4 + 4 * hi);
 #pragma unroll
         for (int j = 0; j < 4; ++j) c[g4 * 4 + j] = v[j];
     }
-}
-template <bool QLANE>
-__device__ __forceinline__ void rel_start(f32x16& s, const i32x16& c, const RelLane<QLANE>& l, int hi, int prefix, int row0) {
     if (l.any) {
         int lim = prefix - row0 - 4 * hi;
         asm volatile("" : "+v"(lim));  // (opaque: 16 lane masks would be hoisted into 32 SGPRs)
@@ -141,12 +138,6 @@ __device__ __forceinline__ void rel_start(f32x16& s, const i32x16& c, const RelL
         for (int e = 0; e < 16; ++e) s[e] = *(lds_float)(uintptr_t)(QLANE ? l.at - c[e] : l.at + c[e]);
     }
 }
-template <bool QLANE>
-__device__ __forceinline__ void rel_tile(f32x16& s, const int* codes, const RelLane<QLANE>& l, int hi, int prefix, int row0) {
-    i32x16 c;
-    rel_codes(c, codes, hi);
-    rel_start(s, c, l, hi, prefix, row0);
-}
 
 // ---- host side
 // Largest slice of offsets that a block of `block` consecutive tokens needs: all codes of the other side plus its own span
@@ -156,7 +147,8 @@ static inline int rel_slice_max(int gh, int gw, int block) {
     const int max_code = (gh - 1) * (2 * gw - 1) + gw - 1;
     const int last = block - 1 < grid - 1 ? block - 1 : grid - 1;
     // a block that starts in column x > 0 spans one row border more than one that starts at 0
-    int span = last + ((last + gw - 1) / gw) * (gw - 1);
+    const int borders = (last + gw - 1) / gw;
+    int span = last + (borders < gh - 1 ? borders : gh - 1) * (gw - 1);
     if (span > max_code) span = max_code;
     return max_code + 2 * span + 4;
 }

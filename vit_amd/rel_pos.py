@@ -46,15 +46,14 @@ class RelPosBuckets:
             if m.shape != (self.indices,):
                 raise ValueError(f"RelPosBuckets: bucket_of has shape {tuple(m.shape)}, expected ({self.indices},)")
             m = m.to(self.device, torch.int64)
-            low, high = (int(v) for v in torch.stack([m.min(), m.max()]).tolist())
-            self.num_buckets = high + 1 if num_buckets is None else int(num_buckets)
-            if low < 0 or high >= self.num_buckets:
-                raise ValueError(f"RelPosBuckets: buckets {low}..{high} outside [0, {self.num_buckets})")
-            self.bucket_of = m.to(torch.int32)
             # the indices sorted by bucket: the order in which the gradient adds a bucket's offsets
             by = torch.sort(m, stable=True)
-            self.by_bucket = by.indices.to(torch.int32)
-            self.bucket_start = torch.searchsorted(by.values, torch.arange(self.num_buckets + 1, device=self.device)).to(torch.int32)
+            self.bucket_of, self.by_bucket = m.to(torch.int32), by.indices.to(torch.int32)
+            self.num_buckets = int(by.values[-1]) + 1 if num_buckets is None else int(num_buckets)
+            self.bucket_start = torch.searchsorted(by.values, torch.arange(max(self.num_buckets, 0) + 1, device=self.device)).to(torch.int32)
+            low, high = by.values[[0, -1]].tolist()  # (waits for all of it: the plan may be used on any stream)
+            if low < 0 or high >= self.num_buckets:
+                raise ValueError(f"RelPosBuckets: buckets {low}..{high} outside [0, {self.num_buckets})")
 
     @classmethod
     def sequence(cls, n: int, num_buckets: int = 32, max_distance: int = 128, bidirectional: bool = True, device="cuda") -> "RelPosBuckets":
