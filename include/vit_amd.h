@@ -268,7 +268,8 @@ int vit_qk_norm_rope_bwd(const vit_qk_norm_config* cfg, const void* qkv, const v
  *   (dy + grid_h - 1) (2 grid_w - 1) + dx + grid_w - 1;
  * three more indices follow the (2 grid_h - 1)(2 grid_w - 1) offsets: prefix query on a grid key, grid query on a prefix key,
  * prefix on prefix. bucket = bucket_of[index], or the index itself when bucket_of is NULL (a bucket outside [0, num_buckets)
- * biases nothing). A table entry below -1e30 masks its pairs; a query left without a key gives zeros. */
+ * biases nothing). A table entry below -1e30 masks its pairs (whose keys and values have to be finite
+ * all the same); a query left without a key gives zeros. */
 typedef struct vit_rel_pos {
     int32_t prefix, grid_h, grid_w; /* 0 <= prefix <= 32; seq = prefix + grid_h * grid_w */
     int32_t num_buckets;

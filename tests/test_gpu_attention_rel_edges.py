@@ -3,7 +3,7 @@ elements, views, other streams, tables with entries that no offset names."""
 import pytest
 import torch
 
-from vit_amd import ops, synth
+from vit_amd import _lib, ops, synth
 from vit_amd._lib import VitError
 from vit_amd.rel_pos import RelPosBuckets
 
@@ -184,3 +184,28 @@ def test_another_stream():
     s.synchronize()
     ref = Ref((qkv.float() * 2).to(BF), table, pl.index(), h, h, None, dh ** -0.5)
     assert ((got.cpu().double() - ref.out).abs() <= SLACK * U * (ref.out_mag + ref.out.abs())).all()
+
+
+@pytest.mark.parametrize("b,grid,h,hk,dh", [(2, (5, 7), 4, 2, 32), (40, (14, 14), 4, 4, 64), (60, (10, 10), 4, 2, 48)])
+def test_gradient_without_the_table(b, grid, h, hk, dh):
+    """d_table NULL: the same dqkv; the workspace it writes ends where it says."""
+    pl = plan(grid, 1, False)
+    n = pl.seq
+    qkv, table = make(b, n, h, hk, dh, pl.num_buckets)
+    x, t = qkv.to(DEV), table.to(DEV)
+    g = synth.normal((b, n, h * dh), 4, "d").to(BF).to(DEV)
+    out, lse = ops.attention_rel_bias_train(x, h, t, pl, num_kv_heads=hk)
+    want, dt = ops.attention_rel_bias_backward(x, out, g, lse, h, t, pl, num_kv_heads=hk)
+    lib, c = _lib.load(), pl._c()
+    need = lib.vit_attention_rel_bwd_workspace_bytes(c, b, h, dh)
+    ws = torch.full((need + 4096,), 77, dtype=torch.uint8, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    for table_grad in (None, torch.empty_like(dt)):
+        got = torch.empty_like(x)
+        _lib.check(lib.vit_attention_rel_bwd(c, x.data_ptr(), t.data_ptr(), None, out.data_ptr(), g.data_ptr(), lse.data_ptr(), got.data_ptr(),
+                                             None if table_grad is None else table_grad.data_ptr(), ws.data_ptr(), need, b, h, hk, dh,
+                                             dh ** -0.5, stream))
+        assert torch.equal(got, want) and (ws[need:] == 77).all()
+        assert table_grad is None or torch.equal(table_grad, dt)
+    assert lib.vit_attention_rel_bwd(c, x.data_ptr(), t.data_ptr(), None, out.data_ptr(), g.data_ptr(), lse.data_ptr(), got.data_ptr(), None,
+                                     ws.data_ptr(), need - 1, b, h, hk, dh, dh ** -0.5, stream) != 0

@@ -378,7 +378,8 @@ int check_cfg(const char* who, const vit_qk_norm_config* c, const void* rope) {
     VIT_REQUIRE(c->dtype == VIT_BF16 || c->dtype == VIT_F32, "%s: bad dtype %d", who, c->dtype);
     VIT_REQUIRE(c->eps > 0.f && c->eps < INFINITY, "%s: eps must be positive and finite", who);
     VIT_REQUIRE(c->rot_dim == 0 || (rope && c->rope_len > 0), "%s: rot_dim %d without a rope table", who, c->rot_dim);
-    VIT_REQUIRE((int64_t)c->batch * c->seq < (1LL << 31), "%s: more than 2^31 - 1 tokens", who);
+    // (a wave's next token, up to 32768 further on, is counted in 32 bits too)
+    VIT_REQUIRE((int64_t)c->batch * c->seq < (1LL << 31) - (1 << 16), "%s: too many tokens", who);
     return VIT_OK;
 }
 bool overlaps(const void* a, const void* b, size_t bytes) {

@@ -478,8 +478,9 @@ def attention_rel_bias(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, b
     """``attention`` with a learned relative position bias: softmax(scale Q K^T + table[bucket(i, j), head]) V.
 
     qkv ``[B, N, (H + 2 Hk) * dh]`` fp32 or bf16 -> ``[B, N, H * dh]``; ``table`` ``[num_buckets, H]`` (entries below -1e30 mask their
-    pairs; a query left without a key gives zeros); ``buckets``: ``rel_pos.RelPosBuckets``; ``lengths``: int32 ``[B]``, tokens in use
-    (rows behind give zeros); ``scale`` defaults to ``dh ** -0.5``."""
+    pairs, whose keys and values have to be finite all the same; a query left without a key gives zeros); ``buckets``:
+    ``rel_pos.RelPosBuckets``; ``lengths``: int32 ``[B]``, tokens in use (rows behind are never read and give zeros); ``scale`` defaults
+    to ``dh ** -0.5``."""
     if _elsewhere(qkv):
         with torch.cuda.device(qkv.device):
             return attention_rel_bias(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale)
