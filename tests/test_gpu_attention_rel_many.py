@@ -139,3 +139,27 @@ def test_graph_replays_equal_eager():
         torch.cuda.synchronize()
         for a, e in zip(captured, step()):
             assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("b,grid,h,hk,dh", [(2, (14, 14), 4, 4, 64), (150, (14, 14), 4, 4, 64), (150, (14, 14), 4, 2, 64), (150, (8, 5), 4, 4, 80)])
+def test_nan_stays_in_its_sample(b, grid, h, hk, dh):
+    """A sample whose last row in use is not finite: rows behind it are zeros all the same, the other samples' results keep their bits."""
+    pl = plan(grid, 1, False)
+    n = pl.seq
+    lens = torch.full((b,), n - 5, dtype=torch.int32, device=DEV)
+    qkv, table = make(b, n, h, hk, dh, pl.num_buckets)
+    g, t = synth.normal((b, n, h * dh), 4, "d").to(BF).to(DEV), table.to(DEV)
+
+    def run(x, fwd):
+        out, lse = ops.attention_rel_bias_train(x, h, t, pl, lengths=lens, num_kv_heads=hk)
+        if fwd is not None:  # the gradient from the same forward but for that sample
+            out, lse = torch.cat([out[:1], fwd[0][1:]]), torch.cat([lse[:1], fwd[1][1:]])
+        return out, lse, ops.attention_rel_bias_backward(x, out, g, lse, h, t, pl, lengths=lens, num_kv_heads=hk)[0]
+
+    clean = run(qkv.to(DEV), None)
+    bad = qkv.clone()
+    bad[0, n - 6] = float("nan")
+    got = run(bad.to(DEV), clean)
+    for p, q in zip(clean, got):
+        assert torch.equal(p[1:], q[1:])
+    assert not got[0][0, n - 5:].any() and not got[2][0, n - 5:].any() and torch.isnan(got[2][0, :n - 5]).any()

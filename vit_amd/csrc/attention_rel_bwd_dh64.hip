@@ -82,9 +82,15 @@ __device__ __forceinline__ void turn_rows(bf16x8 (&f)[4], const bf16x8 (&v)[4], 
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) f[ks] = *(const bf16x8*)(blk + ro[ks]);
 }
-// accumulator (lane = token row, registers = head dims) * mul -> bf16 rows; row0 + 31 may lie behind the resource
-__device__ __forceinline__ void store_rows(const f32x16 (&acc)[2], float mul, __amdgpu_buffer_rsrc_t dst, unsigned char* blk, int row0, int pitch, int lane) {
+// accumulator (lane = token row, registers = head dims) * mul -> bf16 rows, zeros from row nb on; row0 + 31 may lie behind the resource
+__device__ __forceinline__ void store_rows(f32x16 (&acc)[2], float mul, __amdgpu_buffer_rsrc_t dst, unsigned char* blk, int row0, int nb, int pitch, int lane) {
     asm volatile("" : "+v"(lane));
+    if (row0 + 32 > nb && row0 + (lane & 31) >= nb) {  // (not by a factor of 0: they are sums of the last row's values, which may be NaN)
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    }
 #pragma unroll
     for (int d = 0; d < 2; ++d)
 #pragma unroll
@@ -299,7 +305,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         wait_vm<0>();  // Q, dO images (issued a phase ago)
         auto dst = [&](int col) { return head_resource<DH>(a.dqkv + (size_t)b * N * pitch + (size_t)col * (DH * 2), N, pitch); };
-        store_rows(acc1, row < nb ? a.scale : 0.f, dst(h), blk, o0, pitch, lane);
+        store_rows(acc1, a.scale, dst(h), blk, o0, nb, pitch, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f1[0]), "+v"(f1[1]), "+v"(f1[2]), "+v"(f1[3]), "+v"(f2[0]), "+v"(f2[1]), "+v"(f2[2]), "+v"(f2[3])::"memory");
         asm volatile("s_barrier" ::: "memory");  // 2: Q, dO images, the rows' L and delta are whole; K, V images are free
         const bool more = item + 1 < last;
@@ -364,9 +370,8 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             load_rows(item + 1, nnb);
         }
         asm volatile("" ::: "memory");  // (the eight stores stay behind the loads: the counted wait above)
-        const float live = row < nb ? 1.f : 0.f;
-        store_rows(acc1, a.scale * live, dst(H + h), blk, o0, pitch, lane);
-        store_rows(acc2, live, dst(2 * H + h), blk, o0, pitch, lane);
+        store_rows(acc1, a.scale, dst(H + h), blk, o0, nb, pitch, lane);
+        store_rows(acc2, 1.f, dst(2 * H + h), blk, o0, nb, pitch, lane);
         ++item;
         nb = nnb;
     }
