@@ -327,13 +327,13 @@ def rope_table(grid, rot_dim: int, theta: float | None = None, device="cuda") ->
 
 def _elsewhere(t: torch.Tensor) -> bool:
     """whether ``t`` lives on another device than the current one (the calls below then enter it)"""
-    return t.is_cuda and t.device.index != torch.cuda.current_device()
+    return t.is_cuda and t.get_device() != torch._C._cuda_getDevice()  # (a tensor is there, so the device is set up)
 
 
 def _raw_stream(t: torch.Tensor) -> int:
     """The current stream of ``t``'s device as a handle: what ``torch.cuda.current_stream().cuda_stream`` gives, without building
     the Stream object (2.6 us of a 5 us call)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _vec(t, name: str, n: int, ref: torch.Tensor, what: str):
@@ -374,16 +374,18 @@ def _qk_norm_args(qkv, num_heads, num_kv_heads, eps, rope, positions, interleave
     b, n, hk, dh = _packed_heads(qkv, num_heads, num_kv_heads, what)
     rot_dim = rope_len = per_sample = 0
     if rope is not None:
-        if rope.dim() != 3 or rope.shape[2] != 2 or rope.shape[0] == 0:
-            raise ValueError(f"{what}: rope must be [positions, rot_dim / 2, 2], got {tuple(rope.shape)}")
+        shape = rope.shape
+        if len(shape) != 3 or shape[2] != 2 or shape[0] == 0:
+            raise ValueError(f"{what}: rope must be [positions, rot_dim / 2, 2], got {tuple(shape)}")
         rope = _single(_near(rope, "rope", qkv))
-        rope_len, rot_dim = rope.shape[0], 2 * rope.shape[1]
+        rope_len, rot_dim = shape[0], 2 * shape[1]
     if positions is not None:
         if rope is None:
             raise ValueError(f"{what}: positions without a rope table")
-        per_sample = positions.dim() == 2
-        if positions.dtype != torch.int32 or positions.shape != ((b, n) if per_sample else (n,)):
-            raise ValueError(f"{what}: positions must be int32 [{n}] or [{b}, {n}], got {positions.dtype} {tuple(positions.shape)}")
+        shape = positions.shape
+        per_sample = len(shape) == 2
+        if positions.dtype is not torch.int32 or shape != ((b, n) if per_sample else (n,)):
+            raise ValueError(f"{what}: positions must be int32 [{n}] or [{b}, {n}], got {positions.dtype} {tuple(shape)}")
         positions = _near(positions, "positions", qkv).contiguous()
     cfg = _lib.vit_qk_norm_config(b, n, num_heads, hk, dh, _NORM[norm], rot_dim, bool(interleaved), rope_len, per_sample,
                                   dtype_code(qkv.dtype), eps)
@@ -486,7 +488,7 @@ def attention_rel_bias(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, b
             return attention_rel_bias(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale)
     qkv = _dev(qkv, "qkv")
     b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias")
-    out = torch.empty((b, n, num_heads * dh), dtype=qkv.dtype, device=qkv.device)
+    out = qkv.new_empty((b, n, num_heads * dh))
     _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(), None,
                                                  b, num_heads, hk, dh, scale, dtype_code(qkv.dtype), _raw_stream(qkv)))
     return out
@@ -501,7 +503,7 @@ def attention_rel_bias_train(qkv: torch.Tensor, num_heads: int, table: torch.Ten
             return attention_rel_bias_train(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale)
     qkv = _bf16(qkv, "qkv")
     b, n, hk, dh, table, lengths, scale = _rel_args(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale, "attention_rel_bias_train")
-    out = torch.empty((b, n, num_heads * dh), dtype=qkv.dtype, device=qkv.device)
+    out = qkv.new_empty((b, n, num_heads * dh))
     lse = torch.empty((b, num_heads, n), dtype=torch.float32, device=qkv.device)
     _lib.check(_lib.load().vit_attention_rel_fwd(buckets._c(), qkv.data_ptr(), table.data_ptr(), _ptr(lengths), out.data_ptr(),
                                                  lse.data_ptr(), b, num_heads, hk, dh, scale, _lib.VIT_BF16, _raw_stream(qkv)))
