@@ -163,3 +163,28 @@ def test_nan_stays_in_its_sample(b, grid, h, hk, dh):
     for p, q in zip(clean, got):
         assert torch.equal(p[1:], q[1:])
     assert not got[0][0, n - 5:].any() and not got[2][0, n - 5:].any() and torch.isnan(got[2][0, :n - 5]).any()
+
+
+@pytest.mark.parametrize("b", [3, 400])
+@pytest.mark.parametrize("n,dh", [(1, 16), (2, 64), (3, 128), (13, 64), (32, 80)])
+def test_few_keys(b, n, dh):
+    """With one chunk of keys dQ has the roundings of dS and its own alone (bars of test_gpu_attention_rel without the part for the rounded
+    out): with a handful of keys the rest would be the most of it."""
+    h = 4
+    pl = plan((1, n), 0, False)
+    qkv, table = make(b, n, h, h, dh, pl.num_buckets)
+    d_out = synth.normal((b, n, h * dh), 4, "d").to(BF)
+    ref = Ref(qkv, table, pl.index(), h, h, None, dh ** -0.5, d_out)
+    q, t = qkv.to(DEV), table.to(DEV)
+    out, lse = ops.attention_rel_bias_train(q, h, t, pl)
+    dq = ops.attention_rel_bias_backward(q, out, d_out.to(DEV), lse, h, t, pl)[0].cpu().double()[..., :h * dh]
+    e = qkv.double().unflatten(-1, (3 * h, dh)).transpose(1, 2)
+    do = d_out.double().unflatten(-1, (h, dh)).transpose(1, 2)
+    s = e[:, :h] @ e[:, h:2 * h].transpose(-1, -2) * dh ** -0.5 + table.double()[pl.index()].permute(2, 0, 1)
+    p, dp = torch.softmax(s, -1), do @ e[:, 2 * h:].transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    size = p * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True))  # fp32 terms: arguments of exp2 below 64 (2^-18 each)
+    tol = SLACK * U * (ds.abs() @ e[:, h:2 * h].abs()) * dh ** -0.5 + 2.0 ** -16 * (size @ e[:, h:2 * h].abs()) * dh ** -0.5
+    want = ref.dqkv[..., :h * dh]
+    tol = tol.transpose(1, 2).flatten(2) + SLACK * U * want.abs() + 1e-30
+    assert ((dq - want).abs() <= tol).all(), ((dq - want).abs() / tol).max()

@@ -77,10 +77,11 @@ __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsign
     f32x16 s, dp;
     rel_tile(s, (const int*)(buf + BUF - CR * 4), rl, hi, a.geo.prefix, row0);
     if constexpr (MODE == MODE_DQ) {
-        float nd = -oD;
-        if constexpr (DH > 64) asm volatile("" : "+v"(nd));  // (opaque: a block of 16 registers kept for it would be spilled)
+        // (from zero here and for the bias, delta taken off behind the products: what the matrix instructions cut off their sums is then
+        // the same in both, and delta's correction holds it. Started from -delta they left
+        // d_table 1.7e-6 off with 12 x 1001 tokens in 8 buckets, 7e-7 now.)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dp[e] = nd;
+        for (int e = 0; e < 16; ++e) dp[e] = 0.f;
     } else {
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
@@ -107,11 +108,23 @@ __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsign
     bf16x8 xt[DB];
     if constexpr (MODE == MODE_DQ) {
         tr.template read_step<0>(xt, t1);
+        float sum = 0.f;  // (a chunk's terms first: fewer roundings at the size of the row's sum)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL) * dp[e];  // dS^T
-            dsum += s[e];
+            s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL);  // P^T
+            dp[e] -= oD;
+            sum = fmaf(s[e], dp[e], sum);
         }
+        dsum += sum;
+        if (nb <= CR) {
+            // All of the row is here: delta's error leaves dS before it is rounded. (With few keys it is a large part of dS, up to twice
+            // dQ's rounding for 3 keys; with more than a chunk of them it is below a twentieth.)
+            const float err = dsum + __shfl_xor(dsum, 32, 64);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] -= err;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= dp[e];  // dS^T
         const bf16x8 x0 = pack8b(s, 0), x1 = pack8b(s, 1);
 #pragma unroll
         for (int d = 0; d < DB; ++d) acc1[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xt[d], x0, acc1[d], 0, 0, 0);
@@ -390,7 +403,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
                 f32x16 s, dp;
                 rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) dp[e] = D;
+                for (int e = 0; e < 16; ++e) dp[e] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const int off = I::at(t * 32 + r, ks * 2 + hi);
@@ -405,7 +418,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
                         if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(__builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L), dp[e], acc[t][e]);
+                for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(__builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L), dp[e] + D, acc[t][e]);
             }
         }
         b = bn;

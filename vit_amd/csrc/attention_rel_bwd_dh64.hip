@@ -240,9 +240,6 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         turn_rows(f1, nq, blk, ro, lane);
         turn_rows(f2, ng, blk, ro, lane);
         if (row < nb) oD = rowD[row];
-        f32x16 start;  // dP's products start from -delta
-#pragma unroll
-        for (int e = 0; e < 16; ++e) start[e] = -oD;
 #pragma unroll
         for (int d = 0; d < 2; ++d)
 #pragma unroll
@@ -260,7 +257,8 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 }
                 rel_tile(s, codes + key0, la, hi, a.geo.prefix, key0);
                 if (t < 4) stage_qg(item, nb, t);  // (a piece a tile: all at once the CU's memory queue would block the wave)
-                dp = start;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dp[e] = 0.f;  // (delta comes off behind the products, as in the bias launch: the same roundings in both)
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
@@ -278,7 +276,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL) * dp[e];  // dS^T
+                    s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL) * (dp[e] - oD);  // dS^T
                     dsum += s[e];
                 }
 #pragma unroll
