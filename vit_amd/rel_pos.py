@@ -50,8 +50,9 @@ class RelPosBuckets:
             by = torch.sort(m, stable=True)
             self.bucket_of, self.by_bucket = m.to(torch.int32), by.indices.to(torch.int32)
             self.num_buckets = int(by.values[-1]) + 1 if num_buckets is None else int(num_buckets)
-            self.bucket_start = torch.searchsorted(by.values, torch.arange(max(self.num_buckets, 0) + 1, device=self.device)).to(torch.int32)
-            low, high = by.values[[0, -1]].tolist()  # (waits for all of it: the plan may be used on any stream)
+            self.bucket_start = torch.searchsorted(by.values, torch.arange(max(self.num_buckets, 0) + 1, device=self.device), out_int32=True)
+            ends = by.values[::max(self.indices - 1, 1)].tolist()  # (waits for all of it: the plan may be used on any stream)
+            low, high = int(ends[0]), int(ends[-1])
             if low < 0 or high >= self.num_buckets:
                 raise ValueError(f"RelPosBuckets: buckets {low}..{high} outside [0, {self.num_buckets})")
 
