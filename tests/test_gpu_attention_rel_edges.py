@@ -209,3 +209,59 @@ def test_gradient_without_the_table(b, grid, h, hk, dh):
         assert table_grad is None or torch.equal(table_grad, dt)
     assert lib.vit_attention_rel_bwd(c, x.data_ptr(), t.data_ptr(), None, out.data_ptr(), g.data_ptr(), lse.data_ptr(), got.data_ptr(), None,
                                      ws.data_ptr(), need - 1, b, h, hk, dh, dh ** -0.5, stream) != 0
+
+
+@pytest.mark.parametrize("grid,prefix,h,dh", [((1, 4096), 0, 12, 64), ((64, 64), 1, 12, 64), ((1, 4096), 0, 12, 80), ((64, 64), 1, 12, 112)])
+def test_long_with_many_rows(grid, prefix, h, dh):
+    """The kernels for many rows at thousands of tokens, whole and with lengths, against the fp32 form (2^-16 of the magnitudes)."""
+    pl = RelPosBuckets(grid, prefix=prefix, device=DEV)
+    n = pl.seq
+    qkv, table = make(1, n, h, h, dh, pl.num_buckets)
+    x, t = qkv.to(DEV), table.to(DEV)
+    f = x.float()
+    want = ops.attention_rel_bias(f, h, t, pl)
+    mag = ops.attention_rel_bias(torch.cat([f[..., :2 * h * dh], f[..., 2 * h * dh:].abs()], -1), h, t, pl)
+    tol = SLACK * U * (mag + want.abs()) + 2.0 ** -16 * mag
+    assert ((ops.attention_rel_bias(x, h, t, pl).float() - want).abs() <= tol).all()
+    full, part = (torch.tensor([m], dtype=torch.int32, device=DEV) for m in (n, n - 37))
+    assert ((ops.attention_rel_bias(x, h, t, pl, lengths=full).float() - want).abs() <= tol).all()
+    want = ops.attention_rel_bias(f, h, t, pl, lengths=part)
+    mag = ops.attention_rel_bias(torch.cat([f[..., :2 * h * dh], f[..., 2 * h * dh:].abs()], -1), h, t, pl, lengths=part)
+    got = ops.attention_rel_bias(x, h, t, pl, lengths=part).float()
+    assert ((got - want).abs() <= SLACK * U * (mag + want.abs()) + 2.0 ** -16 * mag).all() and not got[:, n - 37:].any()
+
+
+def test_two_graphs():
+    """Two captured steps, replayed in turns without a wait between them, keep out of each other's memory; one is captured at its first call."""
+    def make_step(grid, b, h, dh, seed):
+        pl = plan(grid, 1, True)
+        x = synth.normal((b, pl.seq, 3 * h * dh), seed, "x").to(BF).to(DEV)
+        t = synth.normal((pl.num_buckets, h), seed, "t").to(DEV)
+        g = synth.normal((b, pl.seq, h * dh), seed, "g").to(BF).to(DEV)
+        w = torch.ones(dh, device=DEV)
+
+        def step():
+            y = ops.qk_norm_rope(x, h, w, w)
+            out, lse = ops.attention_rel_bias_train(y, h, t, pl)
+            dy, dt = ops.attention_rel_bias_backward(y, out, g, lse, h, t, pl)
+            return (out, dt) + ops.qk_norm_rope_backward(x, dy, h, w, w)[:3]
+        return step
+
+    steps = [make_step((14, 14), 60, 4, 64, 1), make_step((3, 11), 3, 2, 112, 2)]
+    graphs, outs = [], []
+    for s in steps:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s())
+        graphs.append(g)
+    eager = [s() for s in steps]
+    for _ in range(3):
+        for o in outs:
+            for v in o:
+                v.zero_()
+        for g in graphs + graphs[::-1]:
+            g.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, eager):
+            assert all(torch.equal(a, c) for a, c in zip(o, e))
+        steps[0]()  # (eager work between the replays)
