@@ -335,15 +335,15 @@ __global__ __launch_bounds__(1024) void qk_norm_rope_sum_kernel(const float* __r
     const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
     const int col = blockIdx.x * 16 + c, cols = ns * dh;  // dh is a multiple of 16: every column exists
     float s = 0.f;
-    for (int i0 = 0; i0 < blocks; i0 += 64 * 8) {
-        float v[8];
+    for (int i0 = 0; i0 < blocks; i0 += 64 * 16) {
+        float v[16];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 16; ++k) {
             const int i = i0 + k * 64 + g;
             v[k] = i < blocks ? part[(size_t)i * cols + col] : 0.f;
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s += v[k];
+        for (int k = 0; k < 16; ++k) s += v[k];
     }
     red[g][c] = s;
     __syncthreads();
