@@ -1,0 +1,102 @@
+"""GPU tests of single rows of attention_rel_bias that are unlike the others: rows whose scores all lie far from zero.
+
+A softmax does not change when a number is added to all scores of a row, so rows whose every key carries a large entry of the table (a
+finite mask, say) have ordinary probabilities. The inputs are such that fp32 holds every score exactly (queries of zero, or products of
+small integers that stay below 2^24 with the entry), so the bars of test_gpu_attention_rel hold unchanged."""
+import pytest
+import torch
+
+from vit_amd import ops, synth
+from vit_amd.rel_pos import RelPosBuckets
+
+from .test_gpu_attention_rel import BF, DEV, SLACK, U, Ref
+
+pytestmark = pytest.mark.gpu
+
+ROUTES = [  # b, tokens, h, hk, dh, with lengths: the kernels for few rows, one pass, chunks, chunks with lengths and shared keys
+    (2, 70, 3, 3, 64, False),
+    (1, 33, 3, 3, 128, False),
+    (60, 110, 6, 6, 64, False),
+    (60, 110, 6, 6, 64, True),
+    (60, 110, 6, 6, 80, False),
+    (120, 100, 6, 3, 64, True),
+    (100, 97, 6, 3, 128, False),
+]
+IDS = lambda c: "-".join(str(v) for v in c)  # noqa: E731
+
+
+def far_inputs(route, value, integers):
+    b, n, h, hk, dh, ragged = route
+    pl = RelPosBuckets((1, n), device=DEV)
+    qkv = synth.normal((b, n, (h + 2 * hk) * dh), 9, "qkv")
+    table = synth.normal((pl.num_buckets, h), 9, "table", std=0.8)
+    if integers:
+        qkv[..., :(h + hk) * dh] = qkv[..., :(h + hk) * dh].round().clamp(-2, 2)
+    else:
+        qkv[..., :h * dh] = 0
+    table[n - 1:] = value             # keys at or before the query: the last query has no other
+    table[:, 1][n - 11:n - 1] = value  # second head: only keys more than 10 behind the query are ordinary
+    table[:, 2] = value               # third head: every key
+    ln = torch.tensor([(37 * i * i + 11 * i) % (n + 1) for i in range(b)], dtype=torch.int32) if ragged else None
+    return pl, qkv.to(BF), table, ln
+
+
+def run(route, value, integers, train):
+    b, n, h, hk, dh, ragged = route
+    pl, qkv, table, ln = far_inputs(route, value, integers)
+    d_out = synth.normal((b, n, h * dh), 4, "d_out").to(BF)
+    ref = Ref(qkv, table, pl.index(), h, hk, ln, 0.125, d_out)
+    kw = dict(lengths=None if ln is None else ln.to(DEV), num_kv_heads=hk, scale=0.125)
+    q, t, g = qkv.to(DEV), table.to(DEV), d_out.to(DEV)
+    out, lse = ops.attention_rel_bias_train(q, h, t, pl, **kw)
+    if not train:
+        assert torch.equal(torch.isinf(lse).cpu(), ref.empty)
+        assert ((lse.cpu().double() - ref.lse)[~ref.empty].abs() <= 2.0 ** -18 * (1 + ref.lse[~ref.empty].abs())).all()
+        for got in (out, ops.attention_rel_bias(q, h, t, pl, **kw)):
+            err, tol = (got.cpu().double() - ref.out).abs(), SLACK * U * (ref.out_mag + ref.out.abs()) + 1e-30
+            assert (err <= tol).all(), (err / tol).max()
+        f = ops.attention_rel_bias(q.float(), h, t, pl, **kw)
+        err, tol = (f.cpu().double() - ref.out).abs(), 2.0 ** -16 * ref.out_mag + 1e-30
+        assert (err <= tol).all(), (err / tol).max()
+        return
+    dqkv, dt = ops.attention_rel_bias_backward(q, out, g, lse, h, t, pl, **kw)
+    err, tol = (dqkv.cpu().double() - ref.dqkv).abs(), SLACK * (ref.dmag + U * ref.dqkv.abs()) + 2.0 ** -16 * ref.dqkv.abs().max() + 1e-30
+    assert (err <= tol).all(), (err / tol).max()
+    err, tol = (dt.cpu().double() - ref.dtable).abs(), 2.0 ** -16 * ref.dtable_mag + 1e-30
+    assert (err <= tol).all(), (err / tol).max()
+    again = ops.attention_rel_bias_backward(q, out, g, lse, h, t, pl, **kw)
+    assert torch.equal(dqkv, again[0]) and torch.equal(dt, again[1])
+
+
+VALUES = [-300.0, -1e4, -1e6, -1e9, -1e12, -9e29, 1e9, 1e20]
+
+
+@pytest.mark.parametrize("value", VALUES)
+@pytest.mark.parametrize("route", ROUTES, ids=IDS)
+def test_far_entries_forward(route, value):
+    run(route, value, False, False)
+
+
+@pytest.mark.parametrize("value", [-2.0 ** 10, -2.0 ** 20, 2.0 ** 20])
+@pytest.mark.parametrize("route", ROUTES, ids=IDS)
+def test_far_entries_with_products_forward(route, value):
+    run(route, value, True, False)
+
+
+def test_far_entries_of_two_sizes():
+    """A row whose keys carry two entries, both far from zero: the larger takes all, also where the running maximum meets it last."""
+    n, h = 200, 2
+    pl = RelPosBuckets((1, n), device=DEV)
+    qkv = synth.normal((2, n, 3 * h * 64), 9, "qkv").to(BF)
+    qkv[..., :h * 64] = 0
+    table = torch.full((pl.num_buckets, h), -2e12)
+    table[:n - 100, 0] = -1e12  # keys more than 99 behind the query
+    table[n + 99:, 1] = -1e12   # keys more than 99 before it
+    ref = Ref(qkv, table, pl.index(), h, h, None, 0.125)
+    for b in (1, 40):  # few rows, the ring
+        x = qkv[:1].repeat(b, 1, 1).to(DEV)
+        got = ops.attention_rel_bias(x, h, table.to(DEV), pl)
+        want = ref.out[:1]
+        assert ((got.cpu().double() - want).abs() <= SLACK * U * (ref.out_mag[:1] + want.abs())).all()
+    f = ops.attention_rel_bias(qkv.float().to(DEV), h, table.to(DEV), pl)
+    assert ((f.cpu().double() - ref.out).abs() <= 2.0 ** -16 * ref.out_mag).all()

@@ -23,7 +23,6 @@ struct RelFwdArgs {
 };
 
 constexpr float kDeferLog2 = 6.0f;  // the running max is left alone until a score outgrows it by more than this (base 2)
-constexpr float kFloor = -1e35f;    // a running max never falls below this: masked scores (-inf) then have probability 0
 constexpr int KCH = 32;             // keys of a staged chunk
 constexpr int NWAVE = 4;            // waves of a workgroup
 
@@ -94,7 +93,8 @@ __global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m_run = kFloor, l_run = 0.f;
+    RelLevel level;
+    float l_run = 0.f;
     for (int c = 0; c < nc; ++c) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");  // the chunk is whole; nobody reads the other buffer any more
@@ -124,10 +124,8 @@ __global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <
             for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
             mx = max_across_halves(mx);
             // rescale only when a score outgrows the running max by more than kDeferLog2: P stays <= 2^kDeferLog2 until then
-            const float m_new = fmaxf(m_run, mx * a.scale_log2e);
-            if (__any(m_new > m_run + kDeferLog2)) {
-                const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-                m_run = m_new;
+            if (__any(level.excess(mx, a.scale_log2e) > kDeferLog2)) {
+                const float alpha = level.raise(mx, a.scale_log2e);
                 l_run *= alpha;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -135,9 +133,10 @@ __global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <
                     for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
             }
             float psum = 0.f;
+            level.arguments(s, a.scale_log2e);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - m_run);
+                s[e] = __builtin_amdgcn_exp2f(s[e]);
                 psum += s[e];
             }
             l_run += psum;
@@ -156,7 +155,7 @@ __global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <
     const bool live = q < nb && (l_tot > 0.f || l_tot != l_tot);  // (a NaN row stays one)
     const float inv = 1.0f / l_tot;
     if (q < N) {
-        if (a.lse != nullptr && hi == 0) a.lse[((size_t)b * H + h) * N + q] = live ? m_run + log2f(l_tot) : INFINITY;
+        if (a.lse != nullptr && hi == 0) a.lse[((size_t)b * H + h) * N + q] = live ? level.log_sum(l_tot, a.scale_log2e) : INFINITY;
         const size_t at = ((size_t)b * N + q) * H * DH + (size_t)h * DH;
 #pragma unroll
         for (int d = 0; d < DB; ++d)

@@ -24,7 +24,6 @@ constexpr int NW = 8;        // waves per workgroup
 constexpr int NQ = 4;        // Q DMA pieces per wave and item
 constexpr int QSLOT = 4096;  // one wave's 32 query rows x 128 B
 constexpr float kDeferLog2 = 6.0f;  // the running max is left alone until a score outgrows it by more than this (base 2)
-constexpr float kFloor = -1e35f;    // a running max never falls below this: masked scores (-inf) then have probability 0
 
 struct RelRingArgs {
     const unsigned char* qkv;
@@ -160,7 +159,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
     for (int s = 0; s < R - 1; ++s) dma_next(s);
 
     f32x16 o[2];  // written by the first tile of every item
-    float m_run = 0.f, l_run = 0.f;
+    RelLevel level;
+    float l_run = 0.f;
     int slot = 0, pslot = R - 1;
     bool prev_active = false;  // did this wave store outputs for the previous item
     bool fresh = true;         // the expansion is this item's
@@ -229,13 +229,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
             for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
             mx = max_across_halves(mx);
             if constexpr (FIRST) {
-                m_run = fmaxf(mx * a.scale_log2e, kFloor);
+                level.set(mx, a.scale_log2e);
             } else {
                 // rescale only when a score outgrows the running max by more than kDeferLog2: P stays <= 2^kDeferLog2 until then
-                const float m_new = fmaxf(m_run, mx * a.scale_log2e);
-                if (__any(m_new > m_run + kDeferLog2)) {
-                    const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-                    m_run = m_new;
+                if (__any(level.excess(mx, a.scale_log2e) > kDeferLog2)) {
+                    const float alpha = level.raise(mx, a.scale_log2e);
                     l_run *= alpha;
 #pragma unroll
                     for (int d = 0; d < 2; ++d)
@@ -244,9 +242,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
                 }
             }
             float psum = 0.f;
+            level.arguments(s, a.scale_log2e);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - m_run);
+                s[e] = __builtin_amdgcn_exp2f(s[e]);
                 psum += s[e];
             }
             if constexpr (FIRST) l_run = psum; else l_run += psum;
@@ -281,7 +280,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(4, 4)))
             const bool live = l_tot > 0.f || l_tot != l_tot;  // (a NaN row stays one)
             const float inv = live ? __builtin_amdgcn_rcpf(l_tot) : 0.f;
             if constexpr (LSE) {
-                if (hi == 0 && q0 + r < N) a.lse[((size_t)cur.b * H + cur.h) * N + q0 + r] = live ? m_run + log2f(l_tot) : INFINITY;
+                if (hi == 0 && q0 + r < N) a.lse[((size_t)cur.b * H + cur.h) * N + q0 + r] = live ? level.log_sum(l_tot, a.scale_log2e) : INFINITY;
             }
             // the lane halves trade 8-byte pieces (v_permlane32_swap): every lane stores 8 consecutive head dims, 16 bytes; rows
             // >= N are out of the resource's range

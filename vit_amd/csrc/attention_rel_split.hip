@@ -22,7 +22,6 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float kFloor = -1e35f;  // a running max never falls below this: masked scores (-inf) then have probability 0
 
 struct RelSplitArgs {
     const void* qkv;
@@ -48,7 +47,7 @@ __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
 
 // ---- one tile's softmax step: s in, probabilities out; o rescaled where a row's maximum rose
 template <int DB>
-__device__ __forceinline__ void soft_step(f32x16& s, f32x16 (&o)[DB], float& m_run, float& l_run, int key0, int nb, int hi, float scale_log2e) {
+__device__ __forceinline__ void soft_step(f32x16& s, f32x16 (&o)[DB], RelLevel& level, float& l_run, int key0, int nb, int hi, float scale_log2e) {
     if (key0 + 32 > nb) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -58,10 +57,8 @@ __device__ __forceinline__ void soft_step(f32x16& s, f32x16 (&o)[DB], float& m_r
 #pragma unroll
     for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
     mx = max_across_halves(mx);
-    const float m_new = fmaxf(m_run, mx * scale_log2e);
-    if (__any(m_new > m_run)) {
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-        m_run = m_new;
+    if (__any(level.excess(mx, scale_log2e) > 0.f)) {
+        const float alpha = level.raise(mx, scale_log2e);
         l_run *= alpha;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -69,18 +66,19 @@ __device__ __forceinline__ void soft_step(f32x16& s, f32x16 (&o)[DB], float& m_r
             for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
     }
     float psum = 0.f;
+    level.arguments(s, scale_log2e);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale_log2e, -m_run));
+        s[e] = __builtin_amdgcn_exp2f(s[e]);
         psum += s[e];
     }
     l_run += psum;
 }
 
-// ---- the join. Regions of `region` floats a wave: O^T [DH][32]; ml: [waves][2][32]
+// ---- the join. Regions of `region` floats a wave: O^T [DH][32]; ml: [waves][3][32], the rows' levels (m, M) and sums
 template <typename T, int DH, bool MIXED>  // MIXED: row i of block d is value DB i + d, not 32 d + i
-__device__ __forceinline__ void join(const f32x16 (&o)[(DH + 31) / 32], float m_run, float l_run, float* regions, int region, float* ml, T* out, float* lse,
-                                     int q0, int nb, int N, int row_elems, int wave, int nw, int lane) {
+__device__ __forceinline__ void join(const f32x16 (&o)[(DH + 31) / 32], const RelLevel& level, float l_run, float c, float* regions, int region, float* ml, T* out,
+                                     float* lse, int q0, int nb, int N, int row_elems, int wave, int nw, int lane) {
     const int r = lane & 31, hi = lane >> 5;
     float* mine = regions + (size_t)wave * region;
 #pragma unroll
@@ -92,21 +90,25 @@ __device__ __forceinline__ void join(const f32x16 (&o)[(DH + 31) / 32], float m_
         }
     l_run += __shfl_xor(l_run, 32, 64);
     if (hi == 0) {
-        ml[wave * 64 + r] = m_run;
-        ml[wave * 64 + 32 + r] = l_run;
+        ml[wave * 96 + r] = level.m;
+        ml[wave * 96 + 32 + r] = level.M;
+        ml[wave * 96 + 64 + r] = l_run;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * (DH / 8); i += blockDim.x) {
         const int q = i & 31, d0 = (i >> 5) * 8;
         if (q0 + q >= N) continue;
-        float m = ml[q];
-        for (int w = 1; w < nw; ++w) m = fmaxf(m, ml[w * 64 + q]);
+        RelLevel top;  // the highest of the waves' levels
+        top.m = ml[q], top.M = ml[32 + q];
+        auto above = [&](int w) { return fmaf(ml[w * 96 + 32 + q] - top.M, c, ml[w * 96 + q] - top.m); };
+        for (int w = 1; w < nw; ++w)
+            if (above(w) > 0.f) top.m = ml[w * 96 + q], top.M = ml[w * 96 + 32 + q];
         float l = 0.f, v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
         for (int w = 0; w < nw; ++w) {
-            const float f = __builtin_amdgcn_exp2f(ml[w * 64 + q] - m);
-            l = fmaf(f, ml[w * 64 + 32 + q], l);
+            const float f = __builtin_amdgcn_exp2f(above(w));
+            l = fmaf(f, ml[w * 96 + 64 + q], l);
             const float* p = regions + (size_t)w * region + d0 * 32 + q;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = fmaf(f, p[e * 32], v[e]);
@@ -126,7 +128,7 @@ __device__ __forceinline__ void join(const f32x16 (&o)[(DH + 31) / 32], float m_
             *(f32x4*)dst = a;
             *(f32x4*)(dst + 4) = c;
         }
-        if (lse != nullptr && d0 == 0) lse[q0 + q] = live ? m + log2f(l) : INFINITY;
+        if (lse != nullptr && d0 == 0) lse[q0 + q] = live ? top.log_sum(l, c) : INFINITY;
     }
 }
 
@@ -161,7 +163,7 @@ struct Split {  // what both kernels start with
         regions = (float*)(smem + IMG);
         region = smem + IMG + (size_t)wave * REGION;
         ml = (float*)(smem + IMG + (size_t)nw * REGION);
-        codes = (int*)(ml + nw * 64);
+        codes = (int*)(ml + nw * 96);
         bias = (float*)(codes + ((N + 31) >> 5) * 32);
         b = blockIdx.x / H, h = blockIdx.x - b * H;
         const int hk = h / (H / a.HK);
@@ -206,7 +208,8 @@ __global__ __launch_bounds__(512) void attention_rel_split_bf16_kernel(const Rel
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m_run = kFloor, l_run = 0.f;
+    RelLevel level;
+    float l_run = 0.f;
     for (int t = w.wave; t < w.nt; t += w.nw) {
         f32x16 s;
         rel_tile(s, w.codes + t * 32, w.rl, w.hi, a.geo.prefix, t * 32);
@@ -221,7 +224,7 @@ __global__ __launch_bounds__(512) void attention_rel_split_bf16_kernel(const Rel
             w.tile(w.kr, w.region, t + w.nw);
             w.tile(w.vr, w.region + S::IMG, t + w.nw);
         }
-        soft_step<DB>(s, o, m_run, l_run, t * 32, w.nb, w.hi, a.scale_log2e);
+        soft_step<DB>(s, o, level, l_run, t * 32, w.nb, w.hi, a.scale_log2e);
 #pragma unroll
         for (int sk = 0; sk < 2; ++sk) {
             const bf16x8 pb = pack8(s, sk);
@@ -229,7 +232,7 @@ __global__ __launch_bounds__(512) void attention_rel_split_bf16_kernel(const Rel
             for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt[sk][d], pb, o[d], 0, 0, 0);
         }
     }
-    join<bf16_t, DH, false>(o, m_run, l_run, w.regions, S::REGION / 4, w.ml, (bf16_t*)a.out + ((size_t)w.b * a.N * a.H + w.h) * DH,
+    join<bf16_t, DH, false>(o, level, l_run, a.scale_log2e, w.regions, S::REGION / 4, w.ml, (bf16_t*)a.out + ((size_t)w.b * a.N * a.H + w.h) * DH,
                             a.lse ? a.lse + ((size_t)w.b * a.H + w.h) * a.N : nullptr, w.q0, w.nb, a.N, a.H * DH, w.wave, w.nw, w.lane);
 }
 
@@ -248,7 +251,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DH <= 64 ? 
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m_run = kFloor, l_run = 0.f;
+    RelLevel level;
+    float l_run = 0.f;
     for (int t = w.wave; t < w.nt; t += w.nw) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this tile's keys
         // values: key (e & 3) + 8 (e >> 2) + 4 hi of the tile, what register e of s holds
@@ -286,19 +290,19 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DH <= 64 ? 
         }
         asm volatile("" : "+v"(s));
         if (t + w.nw < w.nt) w.tile(w.kr, w.region, t + w.nw);  // (this tile's reads are over)
-        soft_step<DB>(s, o, m_run, l_run, t * 32, w.nb, w.hi, a.scale_log2e);
+        soft_step<DB>(s, o, level, l_run, t * 32, w.nb, w.hi, a.scale_log2e);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[e][d], s[e], o[d], 0, 0, 0);
     }
-    join<float, DH, true>(o, m_run, l_run, w.regions, S::REGION / 4, w.ml, (float*)a.out + ((size_t)w.b * a.N * a.H + w.h) * DH, nullptr, w.q0,
+    join<float, DH, true>(o, level, l_run, a.scale_log2e, w.regions, S::REGION / 4, w.ml, (float*)a.out + ((size_t)w.b * a.N * a.H + w.h) * DH, nullptr, w.q0,
                           w.nb, a.N, a.H * DH, w.wave, w.nw, w.lane);
 }
 
 // LDS of a workgroup of nw waves, and how many waves fit (one always does)
 size_t split_lds(int dh, int size, int nw, int N, int slice) {
-    return split_image(dh, size) + (size_t)nw * (split_region(dh, size) + 256) + ((size_t)(N + 31) / 32 * 32 + slice) * 4;
+    return split_image(dh, size) + (size_t)nw * (split_region(dh, size) + 384) + ((size_t)(N + 31) / 32 * 32 + slice) * 4;
 }
 int split_waves(int dh, int size, int N, int slice, int most) {
     const int nt = ceil_div(N, 32);

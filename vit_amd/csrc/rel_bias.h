@@ -9,6 +9,7 @@
 // prefix key, prefix on prefix.
 #pragma once
 #include "vit_common.h"
+#include <math.h>
 
 struct RelGeo {
     const float* table;    // [num_buckets, heads]
@@ -138,6 +139,52 @@ __device__ __forceinline__ void rel_tile(f32x16& s, const int* codes, const RelL
         for (int e = 0; e < 16; ++e) s[e] = *(lds_float)(uintptr_t)(QLANE ? l.at - c[e] : l.at + c[e]);
     }
 }
+
+// ---- A row's level: what its probabilities are taken against, p = 2^(s c - level), s a raw score (product + bias / scale), c = scale log2 e.
+// It is held in two parts, level = M c + m. A row has M = 0 and m = its running maximum, rounded: fma(s, c, -m) takes it off the unrounded
+// s c, and what m was rounded by is a factor of the whole row that the sum of the row has too. But that factor is 2^(half an ulp of m): from
+// |m| = 2^31 on it leaves fp32's range (every key of the row at a finite mask of -1e10, say: NaN or zeros). So a row further than kRelFar
+// from zero has M = its raw maximum and m = 0: s - M is exact where p is not small. One subtraction a score, made only where a row of the wave
+// needs it (`far`, wave-uniform).
+constexpr float kRelFloor = -1e35f;    // a level never falls below this: masked scores (-inf) then have probability 0
+constexpr float kRelFar = 16777216.f;  // 2^24: the factor is at most 2^0.5 up to here
+struct RelLevel {
+    float M = 0.f, m = kRelFloor;
+    bool far = false;
+    // how far (base 2) the row's scores, `mx` their largest, rise above the level
+    __device__ __forceinline__ float excess(float mx, float c) const { return fmaf(mx - M, c, -m); }
+    // the level of a row whose largest score so far is `mx`
+    __device__ __forceinline__ void set(float mx, float c) {
+        const float p = mx * c;
+        const bool over = p > kRelFloor, f = over && fabsf(p) > kRelFar;
+        M = f ? mx : 0.f;
+        m = f ? 0.f : over ? p : kRelFloor;
+        far = __any(f);
+    }
+    // raised to `mx` where that is above it (all lanes together); returns the factor of what was summed against the old one
+    __device__ __forceinline__ float raise(float mx, float c) {
+        const bool up = excess(mx, c) > 0.f;
+        const float p = mx * c;
+        const bool f = fabsf(p) > kRelFar;
+        const float M1 = up ? f ? mx : 0.f : M, m1 = up ? f ? 0.f : p : m;
+        const float factor = __builtin_amdgcn_exp2f(fmaf(M - M1, c, m - m1));
+        M = M1;
+        m = m1;
+        far = __any(M != 0.f);
+        return factor;
+    }
+    // scores to exponents' arguments, in place
+    __device__ __forceinline__ void arguments(f32x16& s, float c) const {
+        if (far) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] -= M;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], c, -m);
+    }
+    // base-2 log-sum-exp from the row's sum
+    __device__ __forceinline__ float log_sum(float sum, float c) const { return fmaf(M, c, m + log2f(sum)); }
+};
 
 // ---- host side
 // Largest slice of offsets that a block of `block` consecutive tokens needs: all codes of the other side plus its own span
