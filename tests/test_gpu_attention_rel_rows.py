@@ -100,3 +100,15 @@ def test_far_entries_of_two_sizes():
         assert ((got.cpu().double() - want).abs() <= SLACK * U * (ref.out_mag[:1] + want.abs())).all()
     f = ops.attention_rel_bias(qkv.float().to(DEV), h, table.to(DEV), pl)
     assert ((f.cpu().double() - ref.out).abs() <= 2.0 ** -16 * ref.out_mag).all()
+
+
+@pytest.mark.parametrize("value", VALUES)
+@pytest.mark.parametrize("route", ROUTES, ids=IDS)
+def test_far_entries_gradient(route, value):
+    run(route, value, False, True)
+
+
+@pytest.mark.parametrize("value", [-2.0 ** 10, -2.0 ** 20, 2.0 ** 20])
+@pytest.mark.parametrize("route", ROUTES, ids=IDS)
+def test_far_entries_with_products_gradient(route, value):
+    run(route, value, True, True)

@@ -7,7 +7,8 @@
 //   1 dQ: 32 queries a wave on the lane, keys streamed through LDS. delta from the wave's own rows of dO and O carries the
 //     rounding of O and of the P that made it (about 2^-9), which is nothing beside dQ's own rounding but would stay in the
 //     fp32 sums of dS that make d_table. Rows of the true dS sum to zero (the P of a row sum to 1), so the row sums of the dS
-//     computed with the rounded delta, kept in fp32 beside the products, are its error: delta + sum is written for 2 and 3.
+//     computed with the rounded delta, kept in fp32 beside the products, are its error: delta + sum is written for 2 and 3. Rows whose lse is
+//     far from zero get their statistic again, in two parts (rel_bias.h), before the products: for this launch and for 2 and 3.
 //   2 dK, dV: 32 keys a wave on the lane, the queries of every head of the group streamed through LDS.
 //   3 bias: one block of (query, key) of one head and a range of samples per workgroup. The bias depends on the pair and not on the
 //     sample, and so does the place of dS in its gradient: dS is summed over the samples in registers, and only the sum is folded by
@@ -22,8 +23,8 @@
 
 // launches 1 and 2 in one pass where a head fits the LDS (attention_rel_bwd_dh64.hip)
 bool attention_rel_bwd_dh64_eligible(int N, int heads, int kv_heads, int head_dim);
-int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* ndelta, void* dqkv,
-                                  const int* lengths, int batch, int N, int heads, float scale, hipStream_t stream);
+int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* ndelta, float* rows,
+                                  int* met, void* dqkv, const int* lengths, int batch, int N, int heads, float scale, hipStream_t stream);
 
 namespace {
 
@@ -35,8 +36,10 @@ struct RelBwdArgs {
     const bf16_t* out;
     const bf16_t* dout;
     const float* lse;
-    float* ndelta;  // [B, H, N]: -delta, the start value of dP's products
+    float* ndelta;  // [B, H, N]: -delta
+    float* rows;    // [2][B, H, N]: M and L of the rows (rel_bias.h). One pass: only where lse is far from zero
     bf16_t* dqkv;
+    int* met;      // one pass: [workgroups][8]
     float* part;   // [splits][H][tq][tk][fp]: folded sums of the blocks
     float* doff;   // [H][offsets + 3] (with a map)
     float* dtable;
@@ -47,6 +50,8 @@ struct RelBwdArgs {
     int B, N, H, HK;
     int splits, tq, tk, bq, bk, fp;  // bias gradient: sample ranges, query / key blocks, their sizes, pitch of their sums
     float scale, scale_log2e;
+    __device__ float* row_M(int b, int h) const { return rows + ((size_t)b * H + h) * N; }
+    __device__ float* row_L(int b, int h) const { return rows + ((size_t)(B + b) * H + h) * N; }
 };
 
 __device__ __forceinline__ bf16x8 pack8b(const f32x16& p, int s) {
@@ -61,16 +66,17 @@ __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
     return n < 0 ? 0 : n > N ? N : n;
 }
 
-// Buffers of a chunk of 32 inner rows: two images, (lse, -delta), codes; a multiple of 256 (LdsImage::step)
+// Buffers of a chunk of 32 inner rows: two images, (L, -delta, M) of queries, codes; a multiple of 256 (LdsImage::step)
 constexpr int CR = 32;
 template <int DH, int MODE>
 constexpr int chunk_bytes() { return 2 * CR * LdsImage<DH>::ROW + (MODE == MODE_DKV ? 512 : 256); }
 
-// One chunk's products, for 32 outer rows on the lane: `buf` its buffer (at LDS address img; ro: of the lane's first row piece)
+// One chunk's products, for 32 outer rows on the lane: `buf` its buffer (at LDS address img; ro: of the lane's first row piece). DQ: oL the
+// second part of the row's statistic; far: the wave has rows with a first part, which stands in LDS at Mr (not worth a register)
 template <int DH, int MODE>
 __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsigned char* buf, int img, int ro, const TrRead<DH>& tr,
-                                               const RelLane<MODE == MODE_DQ>& rl, const bf16x8 (&f1)[DH / 16], const bf16x8 (&f2)[DH / 16], float oL,
-                                               float oD, f32x16 (&acc1)[(DH + 31) / 32], f32x16 (&acc2)[(DH + 31) / 32], float& dsum, int row0, int nb,
+                                               const RelLane<MODE == MODE_DQ>& rl, const bf16x8 (&f1)[DH / 16], const bf16x8 (&f2)[DH / 16], bool far,
+                                               const float* Mr, float oL, float oD, f32x16 (&acc1)[(DH + 31) / 32], f32x16 (&acc2)[(DH + 31) / 32], float& dsum, int row0, int nb,
                                                int hi) {
     using I = LdsImage<DH>;
     constexpr int KS = DH / 16, DB = (DH + 31) / 32, IMG = CR * I::ROW, BUF = chunk_bytes<DH, MODE>();
@@ -104,6 +110,21 @@ __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsign
         for (int e = 0; e < 16; ++e)
             if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
     }
+    if constexpr (MODE == MODE_DQ) {
+        if (far) {
+            int tid = threadIdx.x;
+            asm volatile("" : "+v"(tid));
+            const float M = Mr[tid & 31];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] -= M;
+        }
+    } else {
+        const float* const Ms = (const float*)(buf + 2 * IMG + 2 * CR * 4);
+        if (__any(Ms[threadIdx.x & 31] != 0.f)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] -= Ms[(e & 3) + 8 * (e >> 2) + 4 * hi];
+        }
+    }
     const unsigned t1 = (unsigned)img, t2 = t1 + IMG;
     bf16x8 xt[DB];
     if constexpr (MODE == MODE_DQ) {
@@ -111,7 +132,7 @@ __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsign
         float sum = 0.f;  // (a chunk's terms first: fewer roundings at the size of the row's sum)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL);  // P^T
+            s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -oL));  // P^T
             dp[e] -= oD;
             sum = fmaf(s[e], dp[e], sum);
         }
@@ -139,8 +160,8 @@ __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsign
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int e = g4 * 4 + j;
-                s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L[j]);  // P
-                dp[e] *= s[e];                                               // dS
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -L[j]));  // P
+                dp[e] *= s[e];                                                    // dS
             }
         }
         const bf16x8 p0 = pack8b(s, 0), p1 = pack8b(s, 1), d0 = pack8b(dp, 0), d1 = pack8b(dp, 1);
@@ -203,15 +224,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
         fill.chunk(r1, dst, CR, wave, nw, row0, nb - 1, pitch);
         fill.chunk(r2, dst + IMG, CR, wave, nw, row0, nb - 1, MODE == MODE_DQ ? pitch : opitch);
         if constexpr (MODE == MODE_DKV) {
-            if (wave == 0) {  // the queries' lse and -delta
-                const size_t at = ((size_t)b * H + h) * N;
+            if (wave == 0) {  // the queries' L, -delta and M
                 int q = row0 + ln;
                 q = q < nb ? q : nb - 1;
-                const __amdgpu_buffer_rsrc_t rl_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.lse + at), 0, (unsigned)N * 4, 0x00020000);
-                const __amdgpu_buffer_rsrc_t rd_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.ndelta + at), 0, (unsigned)N * 4, 0x00020000);
+                auto row_values = [&](const float* p, int place) {
+                    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (unsigned)N * 4, 0x00020000);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(dst + 2 * IMG + place * CR * 4), 4, q * 4, 0, 0, 0);
+                };
                 if (ln < CR) {
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rl_, LDS_PTR(dst + 2 * IMG), 4, q * 4, 0, 0, 0);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rd_, LDS_PTR(dst + 2 * IMG + CR * 4), 4, q * 4, 0, 0, 0);
+                    row_values(a.row_L(b, h), 0);
+                    row_values(a.ndelta + ((size_t)b * H + h) * N, 1);
+                    row_values(a.row_M(b, h), 2);
                 }
             }
         }
@@ -247,6 +270,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
     rel_expand(a.geo, T, sl, MODE == MODE_DQ, MODE == MODE_DQ ? oh : oh * group);
     const RelLane<MODE == MODE_DQ> rl(a.geo, sl, T, row, N - 1);
     const TrRead<DH> tr(lane);
+    float* const Mr = T + sl.n + sl.span + 3 + wave * 32;
+    bool far = false;  // DQ: the wave has rows of the two-part statistic
+    if constexpr (MODE == MODE_DQ) {
+        const bool f = rel_far(oL);
+        far = __any(f);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");  // T is whole
+        if (far) {
+            float M, L;
+            rel_far_rows<DH>(a.geo, sl, rl, f1, base + (size_t)(H + hk) * DH * 2, pitch, nb, lane, a.scale_log2e, M, L);
+            if (f) oL = L;
+            Mr[r] = f ? M : 0.f;  // (both halves of the wave write it)
+        }
+    }
     const int ro = lds0 + I::at(r, hi);
     f32x16 acc1[DB], acc2[DB];  // DQ: acc1 = dQ^T.  DKV: acc1 = dK^T, acc2 = dV^T
 #pragma unroll
@@ -266,12 +303,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
         if (step + 1 < steps) stage(step + 1, c + 1 == nc ? head + 1 : head, c + 1 == nc ? 0 : c + 1);
         const int img = (step & 1) * BUF, row0 = c * CR;
         const unsigned char* const buf = smem + img;
-        chunk_products<DH, MODE>(a, buf, lds0 + img, ro + img, tr, rl, f1, f2, oL, oD, acc1, acc2, dsum, row0, nb, hi);
+        chunk_products<DH, MODE>(a, buf, lds0 + img, ro + img, tr, rl, f1, f2, far, Mr, oL, oD, acc1, acc2, dsum, row0, nb, hi);
         if (++c == nc) { c = 0; ++head; }
     }
     if constexpr (MODE == MODE_DQ) {
         dsum += __shfl_xor(dsum, 32, 64);
-        if (row < N && hi == 0) a.ndelta[((size_t)b * H + oh) * N + row] = oL < INFINITY ? -(oD + dsum) : 0.f;
+        if (row < N && hi == 0) {
+            a.ndelta[((size_t)b * H + oh) * N + row] = oL < INFINITY ? -(oD + dsum) : 0.f;
+            a.row_M(b, oh)[row] = far ? Mr[r] : 0.f;
+            a.row_L(b, oh)[row] = oL;
+        }
     }
     // ---- store (rows behind the sample's length: zeros)
     if (row < N) {
@@ -383,13 +424,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
     rel_expand(a.geo, T, sl, true, h);
     for (int i = tid; i < ROWS; i += blockDim.x) codes[i] = rel_row_code(a.geo, sl, true, k0 + i);
     const RelLane<true> rl(a.geo, sl, T, q, N - 1);
+    bool far = false;  // the wave has met rows of the two-part statistic
     while (b < b1) {
         const int bn = next_sample(b + 1), nnb = bn < b1 ? sample_length(a.lengths, bn, N) : 0;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // this sample's images are whole; nobody reads the other buffer any more
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) { fq[ks] = nq[ks]; fo[ks] = no[ks]; }
-        L = q < nb ? nL : INFINITY;  // P = exp2(.. - inf) = 0 for rows behind the sample
+        const bool f = rel_far(nL);
+        far |= __any(f);
+        L = q < nb && !f ? nL : INFINITY;  // P = exp2(.. - inf) = 0 for rows behind the sample (and those that come behind the loop)
         D = nD;
         const unsigned char* Kb = smem + buf * 2 * IMG;
 #pragma unroll
@@ -418,12 +462,50 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
                         if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(__builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L), dp[e] + D, acc[t][e]);
+                for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -L)), dp[e] + D, acc[t][e]);
             }
         }
         b = bn;
         nb = nnb;
         buf ^= 1;
+    }
+
+    // ---- rows whose lse is far from zero, against their two-part statistic; slow, from memory (no barrier)
+    if (far) {
+        for (b = next_sample(b0); b < b1; b = next_sample(b + 1)) {
+            nb = sample_length(a.lengths, b, N);
+            L = q < nb ? a.lse[((size_t)b * H + h) * N + q] : INFINITY;
+            const bool f = rel_far(L);
+            if (!__any(f)) continue;
+            load_rows(b, nb, 0, KS);
+            float M = 0.f;
+            L = INFINITY;
+            if (f) {
+                M = a.row_M(b, h)[q];
+                L = a.row_L(b, h)[q];
+            }
+            const unsigned char* kv = (const unsigned char*)a.qkv + (size_t)b * N * pitch + (size_t)(H + hk) * DH * 2 + hi * 16;
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const int key0 = k0 + t * 32;
+                if (key0 >= nb) break;
+                const unsigned char* kp = kv + (size_t)(key0 + r < nb ? key0 + r : nb - 1) * pitch;
+                f32x16 s, dp;
+                rel_tile(s, codes + t * 32, rl, hi, a.geo.prefix, key0);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kp + ks * 32), nq[ks], s, 0, 0, 0);
+                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kp + (size_t)HK * DH * 2 + ks * 32), no[ks], dp, 0, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float x = key0 + (e & 3) + 8 * (e >> 2) + 4 * hi < nb ? fmaf(s[e] - M, a.scale_log2e, -L) : -INFINITY;
+                    acc[t][e] = fmaf(__builtin_amdgcn_exp2f(x), dp[e] + nD, acc[t][e]);
+                }
+            }
+        }
     }
 
     // ---- fold. Each wave its own 32 x 32 tiles through LDS: lane (r, hi) adds the pairs (i, j = (i + r) mod 32), i = 16 hi .. 16 hi + 15,
@@ -611,14 +693,16 @@ __global__ __launch_bounds__(64 * split_waves_most(DH, MODE)) void attn_rel_bwd_
         fill.chunk(r1, buf, CR, 0, 1, row0, nb - 1, pitch);
         fill.chunk(r2, buf + IMG, CR, 0, 1, row0, nb - 1, MODE == MODE_DQ ? pitch : opitch);
         if constexpr (MODE == MODE_DKV) {
-            const size_t at = ((size_t)b * H + h) * N;
             int q = row0 + lane;
             q = q < nb ? q : nb - 1;
-            const __amdgpu_buffer_rsrc_t rl_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.lse + at), 0, (unsigned)N * 4, 0x00020000);
-            const __amdgpu_buffer_rsrc_t rd_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.ndelta + at), 0, (unsigned)N * 4, 0x00020000);
+            auto row_values = [&](const float* p, int place) {
+                const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (unsigned)N * 4, 0x00020000);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(buf + 2 * IMG + place * CR * 4), 4, q * 4, 0, 0, 0);
+            };
             if (lane < CR) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rl_, LDS_PTR(buf + 2 * IMG), 4, q * 4, 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rd_, LDS_PTR(buf + 2 * IMG + CR * 4), 4, q * 4, 0, 0, 0);
+                row_values(a.row_L(b, h), 0);
+                row_values(a.ndelta + ((size_t)b * H + h) * N, 1);
+                row_values(a.row_M(b, h), 2);
             }
         }
         if (lane < CR) *(int*)(buf + BUF - CR * 4 + lane * 4) = rel_row_code(a.geo, sl, MODE == MODE_DQ, row0 + lane);
@@ -658,6 +742,18 @@ __global__ __launch_bounds__(64 * split_waves_most(DH, MODE)) void attn_rel_bwd_
         if (MODE == MODE_DQ && row < nb) oD = d;
         if constexpr (MODE == MODE_DQ) oD += __shfl_xor(oD, 32, 64);
     }
+    float* const Mr = sums + wave * 32;
+    bool far = false;  // DQ: the wave has rows of the two-part statistic
+    if constexpr (MODE == MODE_DQ) {
+        const bool f = rel_far(oL);
+        far = __any(f);
+        if (far) {  // (every wave for itself: they share the queries)
+            float M, L;
+            rel_far_rows<DH>(a.geo, sl, rl, f1, base + (size_t)(H + hk) * DH * 2, pitch, nb, lane, a.scale_log2e, M, L);
+            if (f) oL = L;
+            Mr[r] = f ? M : 0.f;  // (both halves of the wave write it)
+        }
+    }
     f32x16 acc1[DB], acc2[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -672,7 +768,7 @@ __global__ __launch_bounds__(64 * split_waves_most(DH, MODE)) void attn_rel_bwd_
         }
         for (int c = wave; c < nc; c += nw) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            chunk_products<DH, MODE>(a, buf, img, img + I::at(r, hi), tr, rl, f1, f2, oL, oD, acc1, acc2, dsum, c * CR, nb, hi);
+            chunk_products<DH, MODE>(a, buf, img, img + I::at(r, hi), tr, rl, f1, f2, far, Mr, oL, oD, acc1, acc2, dsum, c * CR, nb, hi);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the chunk's reads are over)
             if (c + nw < nc) stage(head0 + g, c + nw);
             else if (g + 1 < nheads) stage(head0 + g + 1, wave);
@@ -681,6 +777,10 @@ __global__ __launch_bounds__(64 * split_waves_most(DH, MODE)) void attn_rel_bwd_
     // ---- the waves' sums
     if constexpr (MODE == MODE_DQ) {
         dsum += __shfl_xor(dsum, 32, 64);
+        if (wave == 0 && hi == 0 && row < N) {
+            a.row_M(b, oh)[row] = far ? Mr[r] : 0.f;
+            a.row_L(b, oh)[row] = oL;
+        }
         if (hi == 0) sums[wave * 32 + r] = dsum;
     }
     float* const part = (float*)smem;  // [nw] of BUF bytes: [DH][32]
@@ -756,12 +856,13 @@ int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, int ncu, hipStream_
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
     VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     if (attn_rel_few_rows((int64_t)items * n32, ncu, false)) return launch_split<DH, MODE>(a, pos, 0, n32, stream);
-    size_t lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)slice * 4;
+    constexpr int kFarRows = MODE == MODE_DQ ? 128 : 0;  // floats behind the expansion
+    size_t lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)(slice + kFarRows) * 4;
     if (!a.lengths && n32 > 4 && n32 % 4 && (int64_t)items * (n32 % 4) <= ncu) {
         // Tiles behind the last whole block of 4 that would start a round of workgroups of their own: by the waves of workgroups instead
         // (4 x 1025 tokens, 16 heads of 80, dK and dV: 131 us with the 33rd tile as a ninth block, 84 + 19 so)
         const int big = rel_slice_max(pos->grid_h, pos->grid_w, 128);
-        const size_t big_lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)big * 4;
+        const size_t big_lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)(big + kFarRows) * 4;
         const int by_lds = (int)(160 * 1024 / big_lds), by_regs = bwd_waves_per_simd(DH, MODE);
         const int64_t slots = (int64_t)ncu * (by_lds < by_regs ? by_lds : by_regs), full = (int64_t)items * (n32 / 4);
         if (big <= kRelSliceCap && (full + items + slots - 1) / slots > (full + slots - 1) / slots) {
@@ -784,7 +885,7 @@ int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, int ncu, hipStream_
 }
 
 struct Workspace {
-    size_t delta, part, doff, bytes;
+    size_t delta, rows, met, part, doff, bytes;
     int splits, tq, tk, bq, bk, fp;
 };
 // LDS of the bias gradient's workgroups: two buffers of K and V images, codes, expansion
@@ -820,7 +921,9 @@ int plan_workspace(const vit_rel_pos* pos, int batch, int heads, int head_dim, W
     w->splits = s < 1 ? 1 : s > batch ? batch : (int)s;
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     w->delta = 0;
-    w->part = up((size_t)batch * heads * N * 4);
+    w->rows = up((size_t)batch * heads * N * 4);
+    w->met = w->rows + up((size_t)batch * heads * N * 8);
+    w->part = w->met + up((size_t)ncu * 8 * 4);
     w->doff = w->part + up((size_t)w->splits * heads * w->tq * w->tk * w->fp * 4);
     w->bytes = w->doff + up((size_t)heads * ((size_t)(2 * pos->grid_h - 1) * (2 * pos->grid_w - 1) + 3) * 4);
     return VIT_OK;
@@ -852,7 +955,7 @@ int launch_all(RelBwdArgs a, const vit_rel_pos* pos, hipStream_t stream) {
     int ncu = 0;
     VIT_TRY_RC(vit_cu_count(&ncu));
     if (attention_rel_bwd_dh64_eligible(a.N, a.H, a.HK, DH) && !attn_rel_few_rows((int64_t)a.B * a.H * ceil_div(a.N, 32), ncu, true)) {
-        VIT_TRY_RC(launch_attention_rel_bwd_dh64(a.geo, a.qkv, a.out, a.dout, a.lse, a.ndelta, a.dqkv, a.lengths, a.B, a.N, a.H, a.scale, stream));
+        VIT_TRY_RC(launch_attention_rel_bwd_dh64(a.geo, a.qkv, a.out, a.dout, a.lse, a.ndelta, a.rows, a.met, a.dqkv, a.lengths, a.B, a.N, a.H, a.scale, stream));
     } else {
         VIT_TRY_RC((launch_part<DH, MODE_DQ>(a, pos, ncu, stream)));
         VIT_TRY_RC((launch_part<DH, MODE_DKV>(a, pos, ncu, stream)));
@@ -911,6 +1014,8 @@ extern "C" int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, co
     a.lse = lse;
     a.dqkv = (bf16_t*)dqkv;
     a.ndelta = (float*)((char*)workspace + w.delta);
+    a.rows = (float*)((char*)workspace + w.rows);
+    a.met = (int*)((char*)workspace + w.met);
     a.part = (float*)((char*)workspace + w.part);
     a.doff = (float*)((char*)workspace + w.doff);
     a.dtable = d_table;

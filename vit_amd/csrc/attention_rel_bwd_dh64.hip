@@ -29,6 +29,8 @@ struct RelBwd64Args {
     const unsigned char* dout;
     const float* lse;
     float* ndelta;
+    float* rows;  // [2][B, H, N]: M and L of rows whose lse is far from zero (rel_bias.h), for the bias sums
+    int* met;     // [grid][8]: whether a workgroup's waves have met such rows
     unsigned char* dqkv;
     const int* lengths;
     RelGeo geo;
@@ -108,6 +110,10 @@ __device__ __forceinline__ void store_rows(f32x16 (&acc)[2], float mul, __amdgpu
     }
 }
 
+// FAR: the launch behind the other, for the items that have rows far from zero: once more, with the two-part statistic and nothing loaded
+// ahead, over what that launch left for them. (A kernel of its own: a branch for such rows anywhere in the other costs it 5 %, this one's
+// early end 3 us.)
+template <bool FAR>
 __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) void attn_rel_bwd_dh64_kernel(const RelBwd64Args a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int N = a.N, H = a.H, B = a.B;
@@ -132,6 +138,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int per = a.nitems / (int)gridDim.x, extra = a.nitems - per * (int)gridDim.x, wg = blockIdx.x;
     const int first = wg * per + (wg < extra ? wg : extra), last = first + per + (wg < extra ? 1 : 0);
     if (first >= last) return;  // uniform
+    if (FAR && !__any((lane & 7) * 64 < (int)blockDim.x && a.met[wg * 8 + (lane & 7)])) return;  // uniform
 
     // ---- lane geometry
     int ro[4];  // row reads: chunk ks * 2 + hi of row r of a tile
@@ -150,6 +157,8 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // stands behind them is not
     const RelSlice sa(a.geo, 0, N - 1, true), sb(a.geo, 0, N - 1, false);
     float* const Tb = T + sa.n + sa.span + 3;
+    float* const rowM = Tb + sb.n + sb.span + 3;  // FAR
+    int* const flags = (int*)(rowM + kRows);       // FAR: of the waves
     const RelLane<true> la(a.geo, sa, T, row, N - 1);
     const RelLane<false> lb(a.geo, sb, Tb, row, N - 1);
     for (int i = tid; i < kRows; i += blockDim.x) {
@@ -199,21 +208,42 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     int item = first, thead = -1;
     auto length_of = [&](int item) { return __builtin_amdgcn_readfirstlane(sample_length(a.lengths, item % B, N)); };
     int nb = length_of(item);
-    for (int i = 0; i < 4; ++i) stage_kv(item, nb, i);
-    load_rows(item, nb);
+    if constexpr (!FAR) {
+        for (int i = 0; i < 4; ++i) stage_kv(item, nb, i);
+        load_rows(item, nb);
+    }
     asm volatile("" ::: "memory");
     wait_vm<0>();
     // (seen as complete here, so that the loop's wait for them counts the stores behind them on every path)
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) asm volatile("" : "+v"(nq[ks]), "+v"(ng[ks]), "+v"(no[ks]));
-    asm volatile("" : "+v"(nL));
+    for (int ks = 0; ks < 4 && !FAR; ++ks) asm volatile("" : "+v"(nq[ks]), "+v"(ng[ks]), "+v"(no[ks]));
+    if constexpr (!FAR) asm volatile("" : "+v"(nL));
     f32x16 acc1[2], acc2[2];
+    bool met = false;
     while (item < last) {
         const int h = item / B, b = item - h * B;
         const int ntb = (nb + 31) >> 5;
         const int nnb = item + 1 < last ? length_of(item + 1) : 0;
-        // this wave's pieces and rows have landed: everything but the previous item's dK / dV stores (8, issued behind them)
-        wait_vm<8>();
+        if constexpr (FAR) {
+            int rw = row;
+            asm volatile("" : "+v"(rw));
+            const bool f = __any(rw < nb && rel_far((a.lse + ((size_t)b * H + h) * N)[rw < nb ? rw : 0]));
+            __syncthreads();  // nobody reads the last item's images any more
+            if (lane == 0) flags[wave] = f;
+            __syncthreads();
+            if (!__any((lane & 7) * 64 < (int)blockDim.x && flags[lane & 7])) {  // uniform
+                ++item;
+                nb = nnb;
+                continue;
+            }
+            for (int i = 0; i < 4; ++i) stage_kv(item, nb, i);
+            load_rows(item, nb);
+            asm volatile("" ::: "memory");
+            wait_vm<0>();
+        } else {
+            // this wave's pieces and rows have landed: everything but the previous item's dK / dV stores (8, issued behind them)
+            wait_vm<8>();
+        }
         asm volatile("s_barrier" ::: "memory");  // 1: K, V images are whole; Q, dO images and T are free
         if (h != thead) {  // uniform
             rel_expand(a.geo, T, sa, true, h);
@@ -226,6 +256,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         // ================= A: dQ
         bf16x8 f1[4], f2[4];
         float oL = row < nb ? nL : INFINITY, oD = 0.f;
+        if constexpr (!FAR) met |= __any(rel_far(oL));
         // delta: dO . O in the rows' own lanes, 8 a row
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -240,6 +271,19 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         turn_rows(f1, nq, blk, ro, lane);
         turn_rows(f2, ng, blk, ro, lane);
         if (row < nb) oD = rowD[row];
+        if constexpr (FAR) {
+            float M, L;
+            rel_far_rows<DH>(a.geo, sa, la, f1, a.qkv + (size_t)b * N * pitch + (size_t)(H + h) * (DH * 2), pitch, nb, lane, a.scale_log2e, M, L);
+            const bool f = rel_far(oL);
+            int rw = row;
+            asm volatile("" : "+v"(rw));  // (opaque here and below, as above)
+            rowM[rw] = f ? M : 0.f;       // (both halves of the wave write it)
+            if (f) {
+                oL = L;
+                a.rows[((size_t)b * H + h) * N + rw] = M;
+                a.rows[((size_t)(B + b) * H + h) * N + rw] = L;
+            }
+        }
 #pragma unroll
         for (int d = 0; d < 2; ++d)
 #pragma unroll
@@ -265,6 +309,13 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], f1[ks], s, 0, 0, 0);
                     dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ks], f2[ks], dp, 0, 0, 0);
                 }
+                if constexpr (FAR) {
+                    int rw = row;
+                    asm volatile("" : "+v"(rw));
+                    const float M = rowM[rw];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] -= M;
+                }
                 bf16x8 kt[2][2];
                 tr_read<0>(kt, tr, (unsigned)tb);
                 if (key0 + 32 > nb) {
@@ -276,7 +327,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - oL) * (dp[e] - oD);  // dS^T
+                    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -oL)) * (dp[e] - oD);  // dS^T
                     dsum += s[e];
                 }
 #pragma unroll
@@ -306,7 +357,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         store_rows(acc1, a.scale, dst(h), blk, o0, nb, pitch, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(f1[0]), "+v"(f1[1]), "+v"(f1[2]), "+v"(f1[3]), "+v"(f2[0]), "+v"(f2[1]), "+v"(f2[2]), "+v"(f2[3])::"memory");
         asm volatile("s_barrier" ::: "memory");  // 2: Q, dO images, the rows' L and delta are whole; K, V images are free
-        const bool more = item + 1 < last;
+        const bool more = !FAR && item + 1 < last;
 
         // ================= B: dK, dV
 #pragma unroll
@@ -327,6 +378,10 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rf[ks], f1[ks], s, 0, 0, 0);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) rf[ks] = *(const bf16x8*)(Gi + tb + ro[ks]);
+                if constexpr (FAR) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] -= rowM[t * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi];
+                }
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
                     const f32x4 Dl = *(const f32x4*)(rowD + t * 32 + 8 * g4 + 4 * hi);
@@ -342,8 +397,8 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int e = g4 * 4 + j;
-                        s[e] = __builtin_amdgcn_exp2f(s[e] * a.scale_log2e - L[j]);  // P
-                        dp[e] *= s[e];                                               // dS
+                        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -L[j]));  // P
+                        dp[e] *= s[e];                                                    // dS
                     }
                 }
                 bf16x8 xt[2][2];
@@ -373,6 +428,7 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         ++item;
         nb = nnb;
     }
+    if (!FAR && lane == 0) a.met[wg * 8 + wave] = met;
 }
 
 }  // namespace
@@ -380,14 +436,16 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // whole heads of 97..224 tokens, as many key as query heads
 bool attention_rel_bwd_dh64_eligible(int N, int heads, int kv_heads, int head_dim) { return head_dim == 64 && heads == kv_heads && N > 96 && N <= 224; }
 
-int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* ndelta, void* dqkv,
-                                  const int* lengths, int batch, int N, int heads, float scale, hipStream_t stream) {
+int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void* out, const void* dout, const float* lse, float* ndelta, float* rows,
+                                  int* met, void* dqkv, const int* lengths, int batch, int N, int heads, float scale, hipStream_t stream) {
     RelBwd64Args a{};
     a.qkv = (const unsigned char*)qkv;
     a.out = (const unsigned char*)out;
     a.dout = (const unsigned char*)dout;
     a.lse = lse;
     a.ndelta = ndelta;
+    a.rows = rows;
+    a.met = met;
     a.dqkv = (unsigned char*)dqkv;
     a.lengths = lengths;
     a.geo = geo;
@@ -399,17 +457,21 @@ int launch_attention_rel_bwd_dh64(const RelGeo& geo, const void* qkv, const void
     a.scale_log2e = scale * LOG2E;
     const int nt = ceil_div(N, 32);
     const size_t lds = (size_t)kRows * (5 * I::ROW + 16) + (size_t)(geo.offsets * 3 + 8) * 4;  // (span <= offsets / 2)
-    VIT_REQUIRE(lds <= 160 * 1024, "attention_rel_bwd: %d offsets do not fit the LDS", geo.offsets);
+    const size_t lds_far = lds + (size_t)(kRows + 8) * 4;
+    VIT_REQUIRE(lds_far <= 160 * 1024, "attention_rel_bwd: %d offsets do not fit the LDS", geo.offsets);
     static PerDeviceInt attr_set;
     std::atomic<int>* as = attr_set.slot();
     if (!as || !as->load(std::memory_order_relaxed)) {
-        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)attn_rel_bwd_dh64_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)attn_rel_bwd_dh64_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        VIT_CHECK_HIP(hipFuncSetAttribute((const void*)attn_rel_bwd_dh64_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (as) as->store(1, std::memory_order_relaxed);
     }
     int ncu = 0;
     VIT_TRY_RC(vit_cu_count(&ncu));
     const int grid = a.nitems < ncu ? a.nitems : ncu;
-    hipLaunchKernelGGL(attn_rel_bwd_dh64_kernel, dim3(grid), dim3(nt * 64), lds, stream, a);
+    hipLaunchKernelGGL(attn_rel_bwd_dh64_kernel<false>, dim3(grid), dim3(nt * 64), lds, stream, a);
+    VIT_CHECK_HIP(hipGetLastError());
+    hipLaunchKernelGGL(attn_rel_bwd_dh64_kernel<true>, dim3(grid), dim3(nt * 64), lds_far, stream, a);
     VIT_CHECK_HIP(hipGetLastError());
     return VIT_OK;
 }

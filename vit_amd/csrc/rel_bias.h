@@ -186,6 +186,50 @@ struct RelLevel {
     __device__ __forceinline__ float log_sum(float sum, float c) const { return fmaf(M, c, m + log2f(sum)); }
 };
 
+// ---- The gradient's probabilities. P = 2^(s c - lse) from the forward's base-2 log-sum-exp is off by the factor 2^(lse's rounding, up to half
+// an ulp) for the whole row: nothing up to |lse| = 2^8 (2^-17), 4 % at a finite mask of -1e6, any factor at -1e9. Rows beyond kRelFarSum
+// therefore have their statistic in two parts, P = 2^((s - M) c - L) with M the row's raw maximum and L = log2 of its sum against M, made anew
+// from the scores where dQ is made and handed to the other launches; every other row has M = 0, L = lse, and its one fma as before.
+constexpr float kRelFarSum = 256.f;
+__device__ __forceinline__ bool rel_far(float lse) { return fabsf(lse) > kRelFarSum && lse < INFINITY; }
+// (M, L) of 32 queries on the lane (fragments qf) over all keys of their sample, read from memory tile by tile: the same instructions in the
+// same order as in the products of the gradient, so the scores are theirs bit for bit (at 1e9 one ulp of a score is a factor of 2^92).
+// One wave, no barrier; `bias` (rl's expansion) is complete.
+template <int DH>
+__device__ __forceinline__ void rel_far_rows(const RelGeo& g, const RelSlice& sl, const RelLane<true>& rl, const bf16x8 (&qf)[DH / 16],
+                                             const unsigned char* keys, int pitch, int nb, int lane, float c, float& M, float& L) {
+    const int r = lane & 31, hi = lane >> 5;
+    float top = -INFINITY, sum = 0.f;
+    for (int key0 = 0; key0 < nb; key0 += 32) {
+        f32x16 s;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int token = key0 + (e & 3) + 8 * (e >> 2) + 4 * hi;
+            const int at = rl.at - (rel_row_code(g, sl, true, token) & rl.mask);
+            s[e] = *(lds_float)(uintptr_t)(token < g.prefix && !rl.mask ? rl.both : at);
+        }
+        const unsigned char* kp = keys + (size_t)(key0 + r < nb ? key0 + r : nb - 1) * pitch + hi * 16;
+#pragma unroll
+        for (int ks = 0; ks < DH / 16; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kp + ks * 32), qf[ks], s, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (key0 + (e & 3) + 8 * (e >> 2) + 4 * hi >= nb) s[e] = -INFINITY;
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+        mx = fmaxf(top, max_across_halves(mx));
+        const float base = mx > -INFINITY ? mx : 0.f;  // (no key so far: every probability 0)
+        float add = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) add += __builtin_amdgcn_exp2f((s[e] - base) * c);
+        sum = fmaf(sum, __builtin_amdgcn_exp2f((top - base) * c), add);
+        top = mx;
+    }
+    sum += __shfl_xor(sum, 32, 64);
+    M = top > -INFINITY ? top : 0.f;
+    L = top > -INFINITY ? log2f(sum) : INFINITY;
+}
+
 // ---- host side
 // Largest slice of offsets that a block of `block` consecutive tokens needs: all codes of the other side plus its own span
 // (floats, with what stands behind the slice)
