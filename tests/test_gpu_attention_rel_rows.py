@@ -1,4 +1,5 @@
-"""GPU tests of single rows of attention_rel_bias that are unlike the others: rows whose scores all lie far from zero.
+"""GPU tests of single rows of attention_rel_bias that are unlike the others: rows whose scores all lie far from zero, rows of a handful of
+keys in a batch of long ones.
 
 A softmax does not change when a number is added to all scores of a row, so rows whose every key carries a large entry of the table (a
 finite mask, say) have ordinary probabilities. The inputs are such that fp32 holds every score exactly (queries of zero, or products of
@@ -112,3 +113,31 @@ def test_far_entries_gradient(route, value):
 @pytest.mark.parametrize("route", ROUTES, ids=IDS)
 def test_far_entries_with_products_gradient(route, value):
     run(route, value, True, True)
+
+
+@pytest.mark.parametrize("b,n,h,hk,dh", [(100, 197, 4, 4, 64), (100, 97, 4, 4, 64), (2, 197, 4, 4, 64), (100, 197, 4, 2, 64)])
+def test_few_keys_of_a_ragged_batch(b, n, h, hk, dh):
+    """Samples of at most one chunk of keys have the dQ that whole sequences of their length have, whatever the batch is padded to: the
+    roundings of dS and its own alone (bars of test_few_keys)."""
+    pl = RelPosBuckets((1, n), device=DEV)
+    ln = torch.tensor([(1, 2, 3, 13, 32)[i % 5] for i in range(b)], dtype=torch.int32)
+    qkv = synth.normal((b, n, (h + 2 * hk) * dh), 9, "qkv").to(BF)
+    table = synth.normal((pl.num_buckets, h), 9, "table", std=0.8)
+    d_out = synth.normal((b, n, h * dh), 4, "d_out").to(BF)
+    q, t, kw = qkv.to(DEV), table.to(DEV), dict(lengths=ln.to(DEV), num_kv_heads=hk)
+    out, lse = ops.attention_rel_bias_train(q, h, t, pl, **kw)
+    dq = ops.attention_rel_bias_backward(q, out, d_out.to(DEV), lse, h, t, pl, **kw)[0].cpu().double()[..., :h * dh]
+    for i in range(b):
+        m = int(ln[i])
+        e = qkv[i, :m].double().unflatten(-1, (h + 2 * hk, dh)).transpose(0, 1)
+        k, v = (x.repeat_interleave(h // hk, 0) for x in (e[h:h + hk], e[h + hk:]))
+        do = d_out[i, :m].double().unflatten(-1, (h, dh)).transpose(0, 1)
+        s = e[:h] @ k.transpose(-1, -2) * dh ** -0.5 + table.double()[pl.index()[:m, :m]].permute(2, 0, 1)
+        p, dp = torch.softmax(s, -1), do @ v.transpose(-1, -2)
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+        size = p * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True))
+        want = (ds @ k * dh ** -0.5).transpose(0, 1).flatten(1)
+        tol = (SLACK * U * ds.abs() + 2.0 ** -16 * size) @ k.abs() * dh ** -0.5
+        tol = tol.transpose(0, 1).flatten(1) + SLACK * U * want.abs() + 1e-30
+        assert ((dq[i, :m] - want).abs() <= tol).all(), (m, ((dq[i, :m] - want).abs() / tol).max())
+        assert not dq[i, m:].any()

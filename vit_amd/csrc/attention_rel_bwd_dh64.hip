@@ -284,6 +284,29 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 a.rows[((size_t)(B + b) * H + h) * N + rw] = L;
             }
         }
+        if (ntb == 1 && o0 < nb) {
+            // One tile of keys: delta's error (the row's sum of dS) leaves delta before dS is made and rounded. (With few keys it is a large
+            // part of dS, up to twice dQ's rounding for 3 keys; with more than a tile of them it is below a twentieth.)
+            f32x16 s, dp;
+            rel_tile(s, codes, la, hi, a.geo.prefix, 0);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Ki + ro[ks]), f1[ks], s, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Vi + ro[ks]), f2[ks], dp, 0, 0, 0);
+            }
+            int rw = row, lim = nb - 4 * hi;
+            asm volatile("" : "+v"(rw), "+v"(lim));
+            const float M = FAR ? rowM[rw] : 0.f;
+            float err = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = (e & 3) + 8 * (e >> 2) < lim ? fmaf(s[e] - M, a.scale_log2e, -oL) : -INFINITY;
+                err = fmaf(__builtin_amdgcn_exp2f(x), dp[e] - oD, err);
+            }
+            oD += err + __shfl_xor(err, 32, 64);
+        }
 #pragma unroll
         for (int d = 0; d < 2; ++d)
 #pragma unroll
@@ -344,7 +367,9 @@ __global__ __launch_bounds__(448) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (hi == 0) {
             rowL[row] = oL;
             rowD[row] = -oD;
-            if (row < N) a.ndelta[((size_t)b * H + h) * N + row] = -oD;
+            int rw = row;
+            if constexpr (FAR) asm volatile("" : "+v"(rw));
+            if (rw < N) a.ndelta[((size_t)b * H + h) * N + rw] = -oD;
         }
         // the wave's own keys for B
 #pragma unroll
