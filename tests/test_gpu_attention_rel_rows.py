@@ -1,5 +1,5 @@
 """GPU tests of single rows of attention_rel_bias that are unlike the others: rows whose scores all lie far from zero, rows of a handful of
-keys in a batch of long ones.
+keys in a batch of long ones, rows that are not finite.
 
 A softmax does not change when a number is added to all scores of a row, so rows whose every key carries a large entry of the table (a
 finite mask, say) have ordinary probabilities. The inputs are such that fp32 holds every score exactly (queries of zero, or products of
@@ -141,3 +141,31 @@ def test_few_keys_of_a_ragged_batch(b, n, h, hk, dh):
         tol = tol.transpose(0, 1).flatten(1) + SLACK * U * want.abs() + 1e-30
         assert ((dq[i, :m] - want).abs() <= tol).all(), (m, ((dq[i, :m] - want).abs() / tol).max())
         assert not dq[i, m:].any()
+
+
+@pytest.mark.parametrize("what", ["q", "v", "d_out"])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("b,grid,prefix,h,hk,dh", [(2, (1, 197), 0, 4, 4, 64), (150, (14, 14), 1, 4, 4, 64), (150, (1, 101), 0, 4, 2, 80), (2, (17, 18), 2, 2, 2, 128)])
+def test_nan_of_a_last_row_stays_with_its_pairs(b, grid, prefix, h, hk, dh, ragged, what):
+    """A last row in use that is not finite: of d_table exactly the entries of its pairs are not finite (with values that are not, all pairs
+    of its sample), those that only rows and keys behind it would reach are."""
+    pl = RelPosBuckets(grid, prefix=prefix, device=DEV)
+    n = pl.seq
+    m = n - 5 if ragged else n
+    kw = dict(lengths=torch.full((b,), m, dtype=torch.int32, device=DEV) if ragged else None, num_kv_heads=hk)
+    qkv = synth.normal((b, n, (h + 2 * hk) * dh), 9, "qkv").to(BF)
+    table = synth.normal((pl.num_buckets, h), 9, "table", std=0.8).to(DEV)
+    d_out = synth.normal((b, n, h * dh), 4, "d_out").to(BF)
+    if what == "q":
+        qkv[0, m - 1, :h * dh] = float("nan")
+    elif what == "v":
+        qkv[0, m - 1, (h + hk) * dh:] = float("nan")
+    else:
+        d_out[0, m - 1] = float("nan")
+    x = qkv.to(DEV)
+    out, lse = ops.attention_rel_bias_train(x, h, table, pl, **kw)
+    dt = ops.attention_rel_bias_backward(x, out, d_out.to(DEV), lse, h, table, pl, **kw)[1]
+    index = pl.index()
+    hit = torch.zeros(pl.num_buckets, dtype=torch.bool)
+    hit[(index[:m, :m] if what == "v" else index[m - 1, :m]).flatten()] = True
+    assert torch.equal(torch.isfinite(dt).cpu(), ~hit[:, None].expand(-1, h))

@@ -433,7 +433,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
         for (int ks = 0; ks < KS; ++ks) { fq[ks] = nq[ks]; fo[ks] = no[ks]; }
         const bool f = rel_far(nL);
         far |= __any(f);
-        L = q < nb && !f ? nL : INFINITY;  // P = exp2(.. - inf) = 0 for rows behind the sample (and those that come behind the loop)
+        L = f ? INFINITY : nL;  // P = exp2(.. - inf) = 0 for rows that come behind the loop
         D = nD;
         const unsigned char* Kb = smem + buf * 2 * IMG;
 #pragma unroll
@@ -454,15 +454,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + off), fq[ks], s, 0, 0, 0);
                     dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(Kb + IMG + off), fo[ks], dp, 0, 0, 0);
                 }
-                if (key0 + 32 > nb) {
-                    int lim = nb - key0 - 4 * hi;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -L));
+                    dp[e] += D;
+                }
+                if (key0 + 32 > nb || (nb < N && q0 + 32 > nb)) {
+                    // pairs behind the sample, chosen and not made zero by P alone: what is made of its last rows may be NaN (queries behind
+                    // the longest sample there can be: once, in the fold)
+                    int lim = q < nb ? nb - key0 - 4 * hi : -64;
                     asm volatile("" : "+v"(lim));
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if ((e & 3) + 8 * (e >> 2) >= lim) s[e] = -INFINITY;
+                    for (int e = 0; e < 16; ++e) {
+                        const bool on = (e & 3) + 8 * (e >> 2) < lim;
+                        s[e] = on ? s[e] : 0.f;
+                        dp[e] = on ? dp[e] : 0.f;
+                    }
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -L)), dp[e] + D, acc[t][e]);
+                for (int e = 0; e < 16; ++e) acc[t][e] = fmaf(s[e], dp[e], acc[t][e]);
             }
         }
         b = bn;
@@ -501,8 +511,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float x = key0 + (e & 3) + 8 * (e >> 2) + 4 * hi < nb ? fmaf(s[e] - M, a.scale_log2e, -L) : -INFINITY;
-                    acc[t][e] = fmaf(__builtin_amdgcn_exp2f(x), dp[e] + nD, acc[t][e]);
+                    const bool on = f && key0 + (e & 3) + 8 * (e >> 2) + 4 * hi < nb;
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[e] - M, a.scale_log2e, -L)), d = dp[e] + nD;
+                    acc[t][e] = fmaf(on ? p : 0.f, on ? d : 0.f, acc[t][e]);
                 }
             }
         }
@@ -531,7 +542,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void a
     for (int t = 0; t < KT; ++t) {
         __builtin_amdgcn_wave_barrier();  // (the last tile's reads come first)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) S[r * 33 + (e & 3) + 8 * (e >> 2) + 4 * hi] = acc[t][e];
+        for (int e = 0; e < 16; ++e) S[r * 33 + (e & 3) + 8 * (e >> 2) + 4 * hi] = q < N ? acc[t][e] : 0.f;
         __builtin_amdgcn_wave_barrier();
         float a10 = 0.f, a11 = 0.f, a20 = 0.f, a21 = 0.f;
         if (q0 < prefix || k0 + t * 32 < prefix) {  // a tile with prefix tokens: those pairs in three sums of their own
