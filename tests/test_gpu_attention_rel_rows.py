@@ -7,7 +7,7 @@ small integers that stay below 2^24 with the entry), so the bars of test_gpu_att
 import pytest
 import torch
 
-from vit_amd import ops, synth
+from vit_amd import _lib, ops, synth
 from vit_amd.rel_pos import RelPosBuckets
 
 from .test_gpu_attention_rel import BF, DEV, SLACK, U, Ref
@@ -169,3 +169,23 @@ def test_nan_of_a_last_row_stays_with_its_pairs(b, grid, prefix, h, hk, dh, ragg
     hit = torch.zeros(pl.num_buckets, dtype=torch.bool)
     hit[(index[:m, :m] if what == "v" else index[m - 1, :m]).flatten()] = True
     assert torch.equal(torch.isfinite(dt).cpu(), ~hit[:, None].expand(-1, h))
+
+
+@pytest.mark.parametrize("grid", [(1, 15872), (89, 89)])
+def test_refused_gradient_writes_nothing(grid):
+    """One size past the limit with d_table: refused, and neither dqkv nor the workspace is touched. Without d_table the call is taken."""
+    pl = RelPosBuckets(grid, device=DEV)
+    n, lib, c = pl.seq, _lib.load(), pl._c()
+    x = synth.normal((1, n, 48), 1, "x").to(BF).to(DEV)
+    t = torch.zeros(pl.num_buckets, 1, device=DEV)
+    out, lse = ops.attention_rel_bias_train(x, 1, t, pl)
+    need = lib.vit_attention_rel_bwd_workspace_bytes(c, 1, 1, 16)
+    ws, dqkv, dt = torch.full((need,), 77, dtype=torch.uint8, device=DEV), torch.full_like(x, 7), torch.full_like(t, 7)
+    args = [x.data_ptr(), t.data_ptr(), None, out.data_ptr(), out.data_ptr(), lse.data_ptr(), dqkv.data_ptr()]
+    rest = [ws.data_ptr(), need, 1, 1, 1, 16, 0.25, torch.cuda.current_stream().cuda_stream]
+    assert lib.vit_attention_rel_bwd(c, *args, dt.data_ptr(), *rest) == -1
+    torch.cuda.synchronize()
+    assert (ws == 77).all() and (dqkv == 7).all() and (dt == 7).all()
+    assert lib.vit_attention_rel_bwd(c, *args, None, *rest) == 0
+    torch.cuda.synchronize()
+    assert torch.isfinite(dqkv.float()).all() and not (dqkv == 7).all()

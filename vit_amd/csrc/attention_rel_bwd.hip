@@ -833,6 +833,8 @@ __global__ __launch_bounds__(64 * split_waves_most(DH, MODE)) void attn_rel_bwd_
     }
 }
 
+// rows of a launch's blocks: equal blocks of up to `most` waves
+int block_rows(int n32, int most) { return ceil_div(n32, ceil_div(n32, most)) * 32; }
 // few enough tiles of 32 rows that the waves of a workgroup share one
 // Whole calls in us, this / the kernels that share inner chunks, 12 heads of 64 (tiles a CU in brackets): 577 tokens, 1 sample [0.9] 42 / 79,
 // 2 [1.8] 65 / 86, 4 [3.6] 107 / 95; against one pass (attention_rel_bwd_dh64.hip) 197 tokens, 1 sample [0.3] 44 / 51, 4 [1.3] 56 / 52;
@@ -863,9 +865,8 @@ int launch_split(const RelBwdArgs& a, const vit_rel_pos* pos, int tile0, int til
 template <int DH, int MODE>
 int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, int ncu, hipStream_t stream) {
     const int n32 = ceil_div(a.N, 32), items = a.B * (MODE == MODE_DQ ? a.H : a.HK);
-    int blocks = ceil_div(n32, 4), waves = ceil_div(n32, blocks), tail = 0;  // equal blocks of up to 4 waves
+    int blocks = ceil_div(n32, 4), waves = block_rows(n32, 4) / 32, tail = 0;
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, waves * 32);
-    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     if (attn_rel_few_rows((int64_t)items * n32, ncu, false)) return launch_split<DH, MODE>(a, pos, 0, n32, stream);
     constexpr int kFarRows = MODE == MODE_DQ ? 128 : 0;  // floats behind the expansion
     size_t lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)(slice + kFarRows) * 4;
@@ -899,7 +900,8 @@ struct Workspace {
     size_t delta, rows, met, part, doff, bytes;
     int splits, tq, tk, bq, bk, fp;
 };
-// LDS of the bias gradient's workgroups: two buffers of K and V images, codes, expansion
+// LDS of the bias gradient's workgroups: two buffers of K and V images, codes, expansion (up to the limit of entries blocks of 2 key tiles
+// fit at every head dim)
 size_t bias_lds(int head_dim, int kt, int slice) {
     const int ch = head_dim / 8, row = (ch == 8 || ch == 16 ? ch : ch + 1) * 16;
     return (size_t)4 * kt * 32 * row + (size_t)(kt * 32 + slice) * 4;
@@ -912,7 +914,7 @@ int plan_workspace(const vit_rel_pos* pos, int batch, int heads, int head_dim, W
     // once a sample) and the head dim leaves the registers room for it (a spilled register's reload waits for all loads under
     // way), else 4 tiles, 2 for head_dim 128 and where the expansion of a long sequence leaves the images less
     w->tq = ceil_div(n32, 8);
-    w->bq = ceil_div(n32, w->tq) * 32;
+    w->bq = block_rows(n32, 8);
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, w->bq);
     w->bk = (head_dim <= 64 && n32 > 4 && n32 <= 7 ? 7 : head_dim <= 112 && bias_lds(head_dim, 4, slice) <= 160 * 1024 ? 4 : 2) * 32;
     // Few samples: blocks of 1, 2 or 4 key tiles, the smallest that gives each CU at most one block and three (block, sample) pairs. us at
@@ -944,11 +946,9 @@ template <int DH, int KT>
 int launch_bias_grad(const RelBwdArgs& a, const vit_rel_pos* pos, hipStream_t stream) {
     const int nw = a.bq / 32;
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, a.bq);
-    VIT_REQUIRE(slice <= kRelSliceCap, "attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     size_t lds = bias_lds(DH, KT, slice);
     const size_t fold = (size_t)nw * (32 * 33 + (KT + 1) * 64 + 3) * 4;
     if (lds < fold) lds = fold;
-    VIT_REQUIRE(lds <= 160 * 1024, "attention_rel_bwd: head_dim %d with %d bias entries does not fit the LDS", DH, slice);
     auto kern = attn_rel_bias_grad_kernel<DH, KT>;
     static PerDeviceInt attr_set;
     std::atomic<int>* as = attr_set.slot();
@@ -1015,6 +1015,9 @@ extern "C" int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, co
     VIT_REQUIRE((int64_t)a.N * (heads + 2 * kv_heads) * head_dim * 2 < (1LL << 31), "vit_attention_rel_bwd: one sample's qkv rows exceed 2 GiB");
     VIT_REQUIRE(!d_table || !pos->bucket_of || (pos->by_bucket && pos->bucket_start),
                 "vit_attention_rel_bwd: the gradient of a mapped table needs the map's inverse");
+    // (every limit before the first launch: a refused call writes nothing)
+    const int slice = rel_slice_max(pos->grid_h, pos->grid_w, block_rows(ceil_div(a.N, 32), d_table ? 8 : 4));
+    VIT_REQUIRE(slice <= kRelSliceCap, "vit_attention_rel_bwd: a %d x %d grid needs %d bias entries at once, %d fit", pos->grid_h, pos->grid_w, slice, kRelSliceCap);
     Workspace w{};
     VIT_TRY_RC(plan_workspace(pos, batch, heads, head_dim, &w));
     if (workspace_bytes < w.bytes)
