@@ -272,7 +272,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
                 int h = h0 + u * HS + slot;
                 asm volatile("" : "+v"(h));  // (opaque: the weights chosen for each of the heads would be kept in registers)
                 const bool isk = h >= a.heads;
-                const float mk = isk ? 1.f : 0.f, mq = 1.f - mk;
                 float x[8], t[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) { x[e] = rx[u].get(e); t[e] = rg[u].get(e); }
@@ -282,11 +281,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void q
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float tx = t[e] * x[e];
-                    sum[0][e] = fmaf(tx, mq, sum[0][e]);
-                    sum[1][e] = fmaf(tx, mk, sum[1][e]);
+                    // (chosen, not times 0 or 1: what is not finite stays with its own sums)
+                    sum[0][e] += isk ? 0.f : tx;
+                    sum[1][e] += isk ? tx : 0.f;
                     if constexpr (LAYER) {
-                        sum[2][e] = fmaf(t[e], mq, sum[2][e]);
-                        sum[3][e] = fmaf(t[e], mk, sum[3][e]);
+                        sum[2][e] += isk ? 0.f : t[e];
+                        sum[3][e] += isk ? t[e] : 0.f;
                     }
                     t[e] *= isk ? w[1][e] : w[0][e];
                     sg += t[e];
