@@ -76,11 +76,21 @@ __device__ __forceinline__ float head_sum(float v) {
     return v;
 }
 
+// a product that is 0 where a factor is, whatever the other one (for finite factors the ordinary one)
+__device__ __forceinline__ float mul_or_zero(float a, float b) {
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
 // what a lane needs to turn its 8 values: cosines and sines of their pairs, and the lane that holds their partners.
 template <int GL, bool IL>
 struct Turn {
-    float c[8], s[8];
+    static constexpr int NC = IL ? 4 : 8;  // (neighbours share theirs)
+    float c[NC], s[NC];
     int partner;  // half-split pairs: lane of the partner values (itself outside the rotated part)
+    int other;    // that lane, itself for a token that is not turned: what is not turned meets no other value, not even times 0 (it may be
+                  // NaN). Neighbours: the multiplication whose product with 0 is 0, whatever the other factor
     __device__ void place(int lane, int chunk, int rot_dim) {
         const int hc = rot_dim >> 4;  // chunks in half the rotated part
         partner = lane;
@@ -88,20 +98,21 @@ struct Turn {
     }
     __device__ void load(const QkArgs& a, int tok, int chunk) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { c[e] = 1.f; s[e] = 0.f; }
+        for (int e = 0; e < NC; ++e) { c[e] = 1.f; s[e] = 0.f; }
+        other = (int)(threadIdx.x & 63);
         if (chunk * 8 >= a.rot_dim) return;
         const int i = tok % a.pos_count;
         const int pos = a.positions ? a.positions[i] : i;
         if (pos < 0 || pos >= a.rope_len) return;  // not turned
+        other = partner;
         const float2* row = a.rope + (size_t)pos * (a.rot_dim >> 1);
         if constexpr (IL) {
             row += chunk * 4;
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
                 const float2 v = row[p];
-                c[2 * p] = c[2 * p + 1] = v.x;
-                s[2 * p] = -v.y;  // even: a cos - b sin; odd: b cos + a sin
-                s[2 * p + 1] = v.y;
+                c[p] = v.x;
+                s[p] = v.y;
             }
         } else {
             const int half = a.rot_dim >> 1;
@@ -120,11 +131,20 @@ struct Turn {
     // sign +1: R y, -1: R^T y (the angle's sign). All lanes call it together.
     template <int SIGN>
     __device__ void apply(float (&y)[8]) const {
-        float o[8];
+        if constexpr (IL) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = IL ? y[e ^ 1] : __shfl(y[e], partner, 64);
+            for (int p = 0; p < 4; ++p) {
+                const float a = y[2 * p], b = y[2 * p + 1], v = SIGN > 0 ? s[p] : -s[p];
+                y[2 * p] = fmaf(a, c[p], -mul_or_zero(v, b));
+                y[2 * p + 1] = fmaf(b, c[p], mul_or_zero(v, a));
+            }
+        } else {
+            float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(SIGN > 0 ? s[e] : -s[e], o[e], y[e] * c[e]);
+            for (int e = 0; e < 8; ++e) o[e] = __shfl(y[e], other, 64);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = fmaf(SIGN > 0 ? s[e] : -s[e], o[e], y[e] * c[e]);
+        }
     }
 };
 
