@@ -79,11 +79,13 @@ typedef struct vit_config {
 
 /* ---- library ---- */
 const char* vit_last_error(void);
-/* ABI version: bumped when an entry point is added or a signature changes. History: 1 = inference path and
- * per-kernel entry points; 2 = + training step, folded LayerNorm, heads, preprocessing, position interpolation,
- * vit_forward_static; 3 = vit_backward_stage accepts any stash that a vit_forward_train of this context filled
- * (several in flight), few-tile GEMM route; the head norm / rotation and relative-position-bias entry points joined it
- * without a change to any earlier signature. The library returns the VIT_ABI_VERSION it was built with. */
+/* ABI version: bumped when the signature or the meaning of a declared entry point changes. Entry points that are only added
+ * leave it (since version 3; the first two were bumped for additions too): whether a library has them, a caller asks by
+ * name (dlsym). History: 1 = inference path and per-kernel entry points; 2 = + training step, folded LayerNorm, heads,
+ * preprocessing, position interpolation, vit_forward_static; 3 = vit_backward_stage accepts any stash that a
+ * vit_forward_train of this context filled (several in flight), few-tile GEMM route. Added to 3: vit_qk_norm_rope_fwd, _bwd,
+ * _bwd_workspace_bytes, vit_attention_rel_fwd, _bwd, _bwd_workspace_bytes, of which a library built earlier has none. The
+ * library returns the VIT_ABI_VERSION it was built with. */
 #define VIT_ABI_VERSION 3
 int vit_abi_version(void);
 
@@ -269,7 +271,9 @@ int vit_qk_norm_rope_bwd(const vit_qk_norm_config* cfg, const void* qkv, const v
  * three more indices follow the (2 grid_h - 1)(2 grid_w - 1) offsets: prefix query on a grid key, grid query on a prefix key,
  * prefix on prefix. bucket = bucket_of[index], or the index itself when bucket_of is NULL (a bucket outside [0, num_buckets)
  * biases nothing). A table entry below -1e30 masks its pairs (whose keys and values have to be finite
- * all the same); a query left without a key gives zeros. */
+ * all the same); a query left without a key gives zeros. Other entries are up to 1e30 in size; a score is an fp32 sum, so a large
+ * entry costs the product beside it its last digits, but the probabilities of a row are those of its scores, however far from
+ * zero all of them lie (a finite mask of -1e4 or -1e9 on every key of a row, say). */
 typedef struct vit_rel_pos {
     int32_t prefix, grid_h, grid_w; /* 0 <= prefix <= 32; seq = prefix + grid_h * grid_w */
     int32_t num_buckets;
@@ -280,13 +284,14 @@ typedef struct vit_rel_pos {
 /* qkv: packed as above (query head h reads key / value head h / (heads / kv_heads)); out [batch * seq, heads * head_dim];
  * lengths: int32 [batch] device, tokens in use of each sample (keys behind are not read, rows behind give zeros), or NULL.
  * lse (VIT_BF16 only, may be NULL): [batch, heads, seq], the base-2 log-sum-exp that the backward takes (+inf where there
- * is no key). A grid too large for the LDS expansion of a query block's offsets (16384 entries:
+ * is no key; of rows beyond +-256 the backward makes the statistic anew, in two parts: two to three times as long where
+ * all rows are such). A grid too large for the LDS expansion of a query block's offsets (16384 entries:
  * beyond 89 x 89, or 1 x 16127 tokens; the backward with d_table, whose blocks are larger, beyond 88 x 88 or 1 x 15871) is refused. */
 int vit_attention_rel_fwd(const vit_rel_pos* pos, const void* qkv, const float* table, const int32_t* lengths, void* out,
                           float* lse, int batch, int heads, int kv_heads, int head_dim, float scale, int dtype,
                           void* stream);
 /* VIT_BF16. dqkv (rows behind a sample's length: zeros) and d_table [num_buckets, heads] fp32, overwritten; d_table may be
- * NULL. No atomics: bitwise reproducible. */
+ * NULL. No atomics: bitwise reproducible. Every refusal comes before the first launch. */
 size_t vit_attention_rel_bwd_workspace_bytes(const vit_rel_pos* pos, int batch, int heads, int head_dim);
 int vit_attention_rel_bwd(const vit_rel_pos* pos, const void* qkv, const float* table, const int32_t* lengths, const void* out,
                           const void* d_out, const float* lse, void* dqkv, float* d_table, void* workspace,

@@ -4,6 +4,10 @@
 //
 // Beyond attention.hip: per-sample lengths (keys behind them are never read, queries behind them give zeros), key / value
 // heads shared by groups of query heads, entries that mask (a query whose every key is masked gives zeros and lse = +inf).
+//
+// Roundings: scores, maxima, sums and the output are fp32. The bf16 kernels round the probabilities to bf16 for the second product (by at most
+// 2^-8 of each: the matrix instructions take bf16 operands; their sum is of the unrounded ones) and the output when it is stored. Against the
+// definition in 64 bits that is 2.3e-3 of the output where rounding the stored output alone leaves 1.7e-3 (fp32 mode: 4e-7).
 #include "lds_image.h"
 #include "rel_bias.h"
 #include <math.h>
@@ -41,8 +45,8 @@ __device__ __forceinline__ int sample_length(const int* lengths, int b, int N) {
 // bf16, any head dim and length. A workgroup of up to 4 waves takes 32 queries a wave of one (sample, head); keys and values come in chunks
 // of 32 by LDS-DMA into two buffers, the next chunk under the products of this one: one barrier a chunk, and three or four workgroups a CU
 // to fill what a wave waits for. Bound by the vector instructions (softmax, bias addresses) that the matrix instructions only partly cover:
-// 4 x 1025 tokens, 16 heads of 80: 69 us, 0.31 PFLOP/s; 6 x 1777 tokens with lengths, 16 heads of 128 over 4 of keys: 153 us. With whole
-// sequences staged, one workgroup a CU, they took 75 and 195 us.
+// 4 x 1025 tokens, 16 heads of 80: 60 us, 0.36 PFLOP/s; 6 samples of up to 1777 tokens, 16 heads of 128 over 4 of keys: 111 to 187 us by their
+// lengths. With whole sequences staged, one workgroup a CU, these took 1.1 and 1.3 times as long.
 template <int DH>
 __global__ __launch_bounds__(64 * NWAVE) __attribute__((amdgpu_waves_per_eu(DH <= 64 ? 4 : 3))) void attention_rel_bf16_kernel(const RelFwdArgs a) {
     using I = LdsImage<DH>;

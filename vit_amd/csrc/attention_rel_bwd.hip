@@ -15,6 +15,9 @@
 //     offset (below) -- no scatter in the loop over samples. P and dP are computed again for it (2 products more).
 //   4 offsets: adds the blocks' folded sums per offset in a fixed order; 5 (only with a map) adds the offsets of a bucket.
 //
+// Roundings: P and dS are rounded to bf16 for the products that make dQ, dK, dV (by at most 2^-8 of each, as P is in the forward: the matrix
+// instructions take bf16 operands), and those when they are stored. d_table is made of the unrounded fp32 dS.
+//
 // Folding: pair (i, j) of a block has linear offset o = i - j, and the grid offset is dx = o mod gw (class 0: x_i >= dx, no row border
 // between) or that - gw (class 1): 2 sums for each diagonal of the block, whatever the grid's width, then three for the prefix classes.
 #include "lds_image.h"
@@ -88,7 +91,7 @@ __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsign
         // d_table 1.7e-6 off with 12 x 1001 tokens in 8 buckets, 7e-7 now.)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = 0.f;
-    } else {
+    } else {  // (from -delta: a cut-off of 2^-24 is nothing beside the rounding of these sums to bf16)
 #pragma unroll
         for (int g4 = 0; g4 < 4; ++g4) {
             const f32x4 Dl = *(const f32x4*)(buf + 2 * IMG + CR * 4 + (8 * g4 + 4 * hi) * 4);
@@ -183,8 +186,8 @@ __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsign
 constexpr int bwd_waves_per_simd(int dh, int mode) { return mode == MODE_DQ ? (dh <= 96 ? 3 : 2) : dh <= 64 ? 3 : dh <= 96 ? 2 : 1; }
 // A workgroup of up to 4 waves takes 32 outer rows a wave of one (sample, head); the inner rows come in chunks of 32 by LDS-DMA into two
 // buffers, the next chunk under the products of this one, in images that serve row reads and transposed reads alike. 4 x 1025 tokens, 16
-// heads of 80: dQ 77 us, dK and dV 84 us, bound by the steps' chains (4400 cycles at three waves a SIMD, 5500 at two, of which the next
-// chunk's loads take 800 to 1300: spread over the products they cost more). Whole sequences staged at once: 118 and 142 us.
+// heads of 80: dQ 71 us, dK and dV 75 us, bound by the steps' chains (4400 cycles at three waves a SIMD, 5500 at two, of which the next
+// chunk's loads take 800 to 1300: spread over the products they cost more). Whole sequences staged at once took 1.5 and 1.7 times as long.
 template <int DH, int MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_per_simd(DH, MODE)))) void attn_rel_bwd_kernel(const RelBwdArgs a) {
     using I = LdsImage<DH>;
@@ -339,9 +342,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
 
 // ---- sums of dS over samples, folded by offset. Grid: (query blocks * key blocks, H, splits). A wave has 32 queries and KT tiles of
 // 32 keys; K and V of the block's keys come by LDS-DMA one sample ahead (two buffers), the wave's own Q and dO rows one sample ahead
-// in registers, so a sample costs one barrier and its loads have a sample's products to land. 256 x 197 tokens, 12 heads of 64: 122 us,
-// 4 x 1025, 16 heads of 80: 103 us (of a workgroup's 80 000 cycles there 17 000 go by before the first product, 10 000 in the fold). Folded a
-// strip of 32 keys at a time by the whole workgroup: 138 and 128 us.
+// in registers, so a sample costs one barrier and its loads have a sample's products to land. 256 x 197 tokens, 12 heads of 64: 116 us,
+// 4 x 1025, 16 heads of 80: 99 us (of a workgroup's 80 000 cycles there 17 000 go by before the first product, 10 000 in the fold). Folded a
+// strip of 32 keys at a time by the whole workgroup it took 1.1 and 1.25 times as long.
 template <int DH, int KT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void attn_rel_bias_grad_kernel(const RelBwdArgs a) {
     using I = LdsImage<DH>;
@@ -836,9 +839,9 @@ __global__ __launch_bounds__(64 * split_waves_most(DH, MODE)) void attn_rel_bwd_
 // rows of a launch's blocks: equal blocks of up to `most` waves
 int block_rows(int n32, int most) { return ceil_div(n32, ceil_div(n32, most)) * 32; }
 // few enough tiles of 32 rows that the waves of a workgroup share one
-// Whole calls in us, this / the kernels that share inner chunks, 12 heads of 64 (tiles a CU in brackets): 577 tokens, 1 sample [0.9] 42 / 79,
-// 2 [1.8] 65 / 86, 4 [3.6] 107 / 95; against one pass (attention_rel_bwd_dh64.hip) 197 tokens, 1 sample [0.3] 44 / 51, 4 [1.3] 56 / 52;
-// 8 heads over 4 of 128, 512 tokens, 1 sample [0.5, 0.25 for dK, dV] 52 / 130
+// Whole calls (replayed) in us, this / the kernels that share inner chunks, 12 heads of 64 (tiles a CU in brackets): 577 tokens, 1 sample [0.9]
+// 44 / 82, 2 [1.8] 68 / 89, 4 [3.6] 110 / 98; against one pass (attention_rel_bwd_dh64.hip) 197 tokens, 1 sample [0.3] 30 / 39, 4 [1.3] 45 / 42;
+// 8 heads over 4 of 128, 512 tokens, 1 sample [0.5, 0.25 for dK, dV] 51 / 131
 bool attn_rel_few_rows(int64_t tiles, int ncu, bool one_pass) { return 2 * tiles <= (one_pass ? 2 : 5) * (int64_t)ncu; }
 
 template <int DH, int MODE>
@@ -872,7 +875,7 @@ int launch_part(const RelBwdArgs& a, const vit_rel_pos* pos, int ncu, hipStream_
     size_t lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)(slice + kFarRows) * 4;
     if (!a.lengths && n32 > 4 && n32 % 4 && (int64_t)items * (n32 % 4) <= ncu) {
         // Tiles behind the last whole block of 4 that would start a round of workgroups of their own: by the waves of workgroups instead
-        // (4 x 1025 tokens, 16 heads of 80, dK and dV: 131 us with the 33rd tile as a ninth block, 84 + 19 so)
+        // (4 x 1025 tokens, 16 heads of 80, dK and dV: 127 us with the 33rd tile as a ninth block, 75 + 19 so)
         const int big = rel_slice_max(pos->grid_h, pos->grid_w, 128);
         const size_t big_lds = (size_t)2 * chunk_bytes<DH, MODE>() + (size_t)(big + kFarRows) * 4;
         const int by_lds = (int)(160 * 1024 / big_lds), by_regs = bwd_waves_per_simd(DH, MODE);
@@ -918,8 +921,8 @@ int plan_workspace(const vit_rel_pos* pos, int batch, int heads, int head_dim, W
     const int slice = rel_slice_max(pos->grid_h, pos->grid_w, w->bq);
     w->bk = (head_dim <= 64 && n32 > 4 && n32 <= 7 ? 7 : head_dim <= 112 && bias_lds(head_dim, 4, slice) <= 160 * 1024 ? 4 : 2) * 32;
     // Few samples: blocks of 1, 2 or 4 key tiles, the smallest that gives each CU at most one block and three (block, sample) pairs. us at
-    // 7 / 4 / 2 / 1 tiles, 12 heads of 64 x 197 tokens: 1 sample 26 / 18 / 13 / 10, 8: 26 / 18 / 16 / 16, 64: 49 / 44 / 48 / 65; 577 tokens
-    // (more blocks than CUs at 2 tiles): 1 sample - / 18 / 22 / 25, 64: - / 268 / 347 / 454
+    // 7 / 4 / 2 / 1 tiles, 12 heads of 64 x 197 tokens: 1 sample 26 / 19 / 13 / 11, 8: 27 / 20 / 16 / 16, 64: 50 / 48 / 52 / 68; 577 tokens
+    // (more blocks than CUs at 2 tiles): 1 sample - / 20 / 25 / 26, 64: - / 274 / 363 / 464
     for (int kt = 1; kt * 32 < w->bk; kt *= 2) {
         const int64_t blocks = (int64_t)heads * w->tq * ceil_div(n32, kt);
         if (blocks <= ncu && blocks * batch <= 3 * (int64_t)ncu) {

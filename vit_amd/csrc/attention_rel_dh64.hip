@@ -8,8 +8,8 @@
 // workgroup meets once or twice, behind a barrier pair of its own.
 //
 // Bound by the waves' own chains (about 140 vector instructions of 4 cycles and 16 exponentials beside 8 matrix instructions a tile, of
-// which a quarter overlap). 256 x 197 tokens, 12 heads: 92 us (310 MB: 3.4 TB/s; attention without a bias 77 us); 32 x 577, 16 heads: 103 us
-// (0.42 PFLOP/s; without 77 us). Whole-sequence images staged at once took 142 and 173 us; the idle eighth wave's place passed round the SIMDs gained
+// which a quarter overlap). 256 x 197 tokens, 12 heads: 89 us (310 MB: 3.5 TB/s; attention without a bias 77 us); 32 x 577, 16 heads: 102 us
+// (0.43 PFLOP/s; without 77 us). Whole-sequence images staged at once took 142 and 173 us; the idle eighth wave's place passed round the SIMDs gained
 // nothing.
 #include "rel_bias.h"
 #include <math.h>
@@ -350,7 +350,7 @@ int launch_ring(const RelRingArgs& a, size_t lds, hipStream_t stream) {
 
 // Takes it: whole sequences of at least 4 key tiles (the counted waits assume an item's stores and Q loads are out of the window
 // before the next item's), one sample's rows within 32-bit offsets, the LDS. us, this / the chunked kernel of attention_rel.hip: 256 x 197
-// tokens x 12 heads 92 / 115, 16 x 1024 x 16 107 / 121, 32 x 577 x 16 103 / 103.
+// tokens x 12 heads 86 / 108, 16 x 1024 x 16 102 / 117, 32 x 577 x 16 97 / 95.
 bool attention_rel_dh64_eligible(const vit_rel_pos* pos, int batch, int heads, int kv_heads) {
     const int N = pos->prefix + pos->grid_h * pos->grid_w;
     if (N <= 96 || (long)N * (heads + 2 * kv_heads) * DH * 2 >= (1L << 31)) return false;

@@ -8,13 +8,13 @@
 // fp32 is bound by the matrix instructions (64 cycles for 4096 operations).
 //
 // Which calls, measured in us, this kernel / the shared ones (bf16; workgroups here per CU in brackets):
-//   197 tokens x 12 heads x 64   samples 1 [0.3]: 5.9 / 11.8   4 [1.3]: 7.3 / 12.0   8 [2.6]: 8.7 / 12.2   16 [5.3]: 14.0 / 12.8
-//   1025 x 16 x 80               samples 1 [2.1]: 32 / 44      2 [4.1]: 50 / 52      4 [8.3]: 92 / 63
-//   256 x 8 x 128                samples 8 [2]: 10.6 / 16.0    16 [4]: 18.4 / 17.4
+//   197 tokens x 12 heads x 64   samples 1 [0.3]: 6.4 / 11.7   4 [1.3]: 7.8 / 11.8   8 [2.6]: 9.2 / 12.1   16 [5.3]: 15.5 / 12.4
+//   1025 x 16 x 80               samples 1 [2.1]: 32 / 45      2 [4.1]: 49 / 48      4 [8.3]: 85 / 60
+//   256 x 8 x 128                samples 8 [2]: 10.8 / 16.6    16 [4]: 19.2 / 18.0
 // so up to 4 a CU. Waves of a workgroup: 8 while there is a CU for each, else 4, more of which fit a CU at once (us at 8 / 4 waves):
-//   bf16 197 x 12 x 64, samples 1: 5.9 / 6.3, 8: 11.1 / 8.7;  577 x 12 x 64, samples 1: 8.1 / 9.4, 8: 34 / 31
-//   fp32 197 x 12 x 64, samples 1: 9.8 / 10.1, 4: 17.5 / 15.1, 32: 94 / 68;  577, samples 16: 258 / 189 (its matrix instructions: 115)
-// fp32 against 128 to 256 queries on shared keys: 197 tokens, samples 4: 15 / 47, 32: 68 / 89; 577, samples 32: 366 / 678.
+//   bf16 197 x 12 x 64, samples 1: 6.4 / 6.7, 8: 11.8 / 9.2;  577 x 12 x 64, samples 1: 8.4 / 9.8, 8: 35 / 32
+//   fp32 197 x 12 x 64, samples 1: 10.2 / 10.5, 4: 18.0 / 15.3, 32: 97 / 69;  577, samples 16: 258 / 189 (its matrix instructions: 115)
+// fp32 with 128 to 256 queries on shared keys took 3 times as long for 4 x 197 tokens, 1.3 for 32 x 197, 1.8 for 32 x 577.
 #include "lds_image.h"
 #include "rel_bias.h"
 #include <math.h>

@@ -480,7 +480,8 @@ def attention_rel_bias(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, b
     """``attention`` with a learned relative position bias: softmax(scale Q K^T + table[bucket(i, j), head]) V.
 
     qkv ``[B, N, (H + 2 Hk) * dh]`` fp32 or bf16 -> ``[B, N, H * dh]``; ``table`` ``[num_buckets, H]`` (entries below -1e30 mask their
-    pairs, whose keys and values have to be finite all the same; a query left without a key gives zeros); ``buckets``:
+    pairs, whose keys and values have to be finite all the same; a query left without a key gives zeros; others up to 1e30 in size,
+    also where every key of a query carries one: a finite mask is a number like any other); ``buckets``:
     ``rel_pos.RelPosBuckets``; ``lengths``: int32 ``[B]``, tokens in use (rows behind are never read and give zeros); ``scale`` defaults
     to ``dh ** -0.5``."""
     if _elsewhere(qkv):
@@ -497,7 +498,7 @@ def attention_rel_bias(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, b
 def attention_rel_bias_train(qkv: torch.Tensor, num_heads: int, table: torch.Tensor, buckets, lengths: torch.Tensor | None = None,
                              num_kv_heads: int | None = None, scale: float | None = None):
     """``attention_rel_bias`` (bf16) that also returns what its backward needs: ``(out, saved)``, ``saved`` the base-2 log-sum-exp of
-    every row ``[B, H, N]`` (+inf where a query has no key)."""
+    every row ``[B, H, N]`` (+inf where a query has no key; the backward makes the statistic of rows beyond +-256 anew)."""
     if _elsewhere(qkv):
         with torch.cuda.device(qkv.device):
             return attention_rel_bias_train(qkv, num_heads, table, buckets, lengths, num_kv_heads, scale)
