@@ -10,7 +10,7 @@ import torch
 from vit_amd import _lib, ops, synth
 from vit_amd.rel_pos import RelPosBuckets
 
-from .test_gpu_attention_rel import BF, DEV, SLACK, U, Ref
+from .test_gpu_attention_rel import BF, DEV, SLACK, U, Ref, plan
 
 pytestmark = pytest.mark.gpu
 
@@ -44,8 +44,11 @@ def far_inputs(route, value, integers):
 
 def run(route, value, integers, train):
     b, n, h, hk, dh, ragged = route
-    pl, qkv, table, ln = far_inputs(route, value, integers)
-    d_out = synth.normal((b, n, h * dh), 4, "d_out").to(BF)
+    compare(*far_inputs(route, value, integers), h, hk, dh, train)
+
+
+def compare(pl, qkv, table, ln, h, hk, dh, train):
+    d_out = synth.normal((*qkv.shape[:2], h * dh), 4, "d_out").to(BF)
     ref = Ref(qkv, table, pl.index(), h, hk, ln, 0.125, d_out)
     kw = dict(lengths=None if ln is None else ln.to(DEV), num_kv_heads=hk, scale=0.125)
     q, t, g = qkv.to(DEV), table.to(DEV), d_out.to(DEV)
@@ -113,6 +116,23 @@ def test_far_entries_gradient(route, value):
 @pytest.mark.parametrize("route", ROUTES, ids=IDS)
 def test_far_entries_with_products_gradient(route, value):
     run(route, value, True, True)
+
+
+@pytest.mark.parametrize("value", [-2.0 ** 20, 2.0 ** 18, -2.0 ** 9])
+@pytest.mark.parametrize("b,grid,prefix,h,hk,dh,mapped,ragged", [
+    (2, (7, 9), 2, 4, 2, 48, True, False), (3, (14, 14), 1, 4, 4, 64, False, True), (60, (10, 11), 32, 6, 6, 64, False, False),
+    (60, (10, 11), 1, 6, 6, 64, True, True), (60, (9, 11), 5, 6, 3, 80, False, True), (70, (5, 13), 1, 8, 4, 128, True, False),
+    (1, (24, 24), 1, 4, 4, 64, False, False), (60, (3, 3), 2, 8, 8, 32, False, True)])
+def test_far_tables_on_a_grid(b, grid, prefix, h, hk, dh, mapped, ragged, value):
+    """Every entry far from zero, each at its own distance, prefix tokens' entries among them; products of small integers."""
+    pl = plan(grid, prefix, mapped)
+    n = pl.seq
+    qkv = synth.normal((b, n, (h + 2 * hk) * dh), 9, "qkv")
+    qkv[..., :(h + hk) * dh] = qkv[..., :(h + hk) * dh].round().clamp(-2, 2)
+    table = value + synth.normal((pl.num_buckets, h), 9, "table", std=2.0).round()
+    ln = torch.tensor([(37 * i * i + 11 * i) % (n + 1) for i in range(b)], dtype=torch.int32) if ragged else None
+    compare(pl, qkv.to(BF), table, ln, h, hk, dh, True)
+    compare(pl, qkv.to(BF), table, ln, h, hk, dh, False)
 
 
 @pytest.mark.parametrize("b,n,h,hk,dh", [(100, 197, 4, 4, 64), (100, 97, 4, 4, 64), (2, 197, 4, 4, 64), (100, 197, 4, 2, 64)])
@@ -189,3 +209,34 @@ def test_refused_gradient_writes_nothing(grid):
     assert lib.vit_attention_rel_bwd(c, *args, None, *rest) == 0
     torch.cuda.synchronize()
     assert torch.isfinite(dqkv.float()).all() and not (dqkv == 7).all()
+
+
+@pytest.mark.parametrize("b,n,h,hk,dh", [(60, 110, 6, 6, 64), (2, 70, 3, 3, 64), (100, 97, 6, 3, 128)])
+def test_far_rows_come_and_go_in_a_graph(b, n, h, hk, dh):
+    """A captured step whose table gets and loses entries far from zero between its replays, against the eager call each time."""
+    pl = RelPosBuckets((1, n), device=DEV)
+    x = synth.normal((b, n, (h + 2 * hk) * dh), 9, "qkv").to(BF).to(DEV)
+    t = synth.normal((pl.num_buckets, h), 9, "table", std=0.8).to(DEV)
+    g = synth.normal((b, n, h * dh), 4, "d_out").to(BF).to(DEV)
+
+    def step():
+        out, lse = ops.attention_rel_bias_train(x, h, t, pl, num_kv_heads=hk)
+        return (out, lse) + ops.attention_rel_bias_backward(x, out, g, lse, h, t, pl, num_kv_heads=hk)
+
+    step()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    ordinary = t.clone()
+    for value in (None, -1e9, None, 1e12, -400.0, None):
+        t.copy_(ordinary)
+        if value is not None:
+            t[n - 1:, 1] = value
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, e in zip(captured, step()):
+            assert torch.equal(a, e) and torch.isfinite(e.float()).all()
