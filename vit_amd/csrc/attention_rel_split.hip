@@ -8,12 +8,12 @@
 // fp32 is bound by the matrix instructions (64 cycles for 4096 operations).
 //
 // Which calls, measured in us, this kernel / the shared ones (bf16; workgroups here per CU in brackets):
-//   197 tokens x 12 heads x 64   samples 1 [0.3]: 6.4 / 11.7   4 [1.3]: 7.8 / 11.8   8 [2.6]: 9.2 / 12.1   16 [5.3]: 15.5 / 12.4
+//   197 tokens x 12 heads x 64   samples 1 [0.3]: 6.5 / 11.7   4 [1.3]: 7.6 / 11.8   8 [2.6]: 9.1 / 12.1   16 [5.3]: 15.5 / 12.4
 //   1025 x 16 x 80               samples 1 [2.1]: 32 / 45      2 [4.1]: 49 / 48      4 [8.3]: 85 / 60
-//   256 x 8 x 128                samples 8 [2]: 10.8 / 16.6    16 [4]: 19.2 / 18.0
+//   256 x 8 x 128                samples 8 [2]: 10.7 / 16.6    16 [4]: 18.8 / 18.0
 // so up to 4 a CU. Waves of a workgroup: 8 while there is a CU for each, else 4, more of which fit a CU at once (us at 8 / 4 waves):
-//   bf16 197 x 12 x 64, samples 1: 6.4 / 6.7, 8: 11.8 / 9.2;  577 x 12 x 64, samples 1: 8.4 / 9.8, 8: 35 / 32
-//   fp32 197 x 12 x 64, samples 1: 10.2 / 10.5, 4: 18.0 / 15.3, 32: 97 / 69;  577, samples 16: 258 / 189 (its matrix instructions: 115)
+//   bf16 197 x 12 x 64, samples 1: 6.5 / 6.7, 8: 11.8 / 9.1;  577 x 12 x 64, samples 1: 8.4 / 9.8, 8: 35 / 32
+//   fp32 197 x 12 x 64, samples 1: 10.2 / 10.5, 4: 18.0 / 15.3, 32: 97 / 68;  577, samples 16: 258 / 186 (its matrix instructions: 115)
 // fp32 with 128 to 256 queries on shared keys took 3 times as long for 4 x 197 tokens, 1.3 for 32 x 197, 1.8 for 32 x 577.
 #include "lds_image.h"
 #include "rel_bias.h"
@@ -75,7 +75,7 @@ __device__ __forceinline__ void soft_step(f32x16& s, f32x16 (&o)[DB], RelLevel& 
     l_run += psum;
 }
 
-// ---- the join. Regions of `region` floats a wave: O^T [DH][32]; ml: [waves][3][32], the rows' levels (m, M) and sums
+// ---- the join. Regions of `region` floats a wave: O^T [DH][32]; ml: [waves][32] of (m, M, sum, -), the rows' levels and sums
 template <typename T, int DH, bool MIXED>  // MIXED: row i of block d is value DB i + d, not 32 d + i
 __device__ __forceinline__ void join(const f32x16 (&o)[(DH + 31) / 32], const RelLevel& level, float l_run, float c, float* regions, int region, float* ml, T* out,
                                      float* lse, int q0, int nb, int N, int row_elems, int wave, int nw, int lane) {
@@ -90,25 +90,29 @@ __device__ __forceinline__ void join(const f32x16 (&o)[(DH + 31) / 32], const Re
         }
     l_run += __shfl_xor(l_run, 32, 64);
     if (hi == 0) {
-        ml[wave * 96 + r] = level.m;
-        ml[wave * 96 + 32 + r] = level.M;
-        ml[wave * 96 + 64 + r] = l_run;
+        *(f32x4*)(ml + (wave * 32 + r) * 4) = f32x4{level.m, level.M, l_run, 0.f};
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * (DH / 8); i += blockDim.x) {
         const int q = i & 31, d0 = (i >> 5) * 8;
         if (q0 + q >= N) continue;
+        auto row = [&](int w) { return *(const f32x4*)(ml + (w * 32 + q) * 4); };
         RelLevel top;  // the highest of the waves' levels
-        top.m = ml[q], top.M = ml[32 + q];
-        auto above = [&](int w) { return fmaf(ml[w * 96 + 32 + q] - top.M, c, ml[w * 96 + q] - top.m); };
-        for (int w = 1; w < nw; ++w)
-            if (above(w) > 0.f) top.m = ml[w * 96 + q], top.M = ml[w * 96 + 32 + q];
+        top.m = row(0)[0], top.M = row(0)[1];
+        auto above = [&](const f32x4& v) { return fmaf(v[1] - top.M, c, v[0] - top.m); };
+        for (int w = 1; w < nw; ++w) {
+            const f32x4 v = row(w);
+            const bool higher = above(v) > 0.f;
+            top.m = higher ? v[0] : top.m;
+            top.M = higher ? v[1] : top.M;
+        }
         float l = 0.f, v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.f;
         for (int w = 0; w < nw; ++w) {
-            const float f = __builtin_amdgcn_exp2f(above(w));
-            l = fmaf(f, ml[w * 96 + 64 + q], l);
+            const f32x4 x = row(w);
+            const float f = __builtin_amdgcn_exp2f(above(x));
+            l = fmaf(f, x[2], l);
             const float* p = regions + (size_t)w * region + d0 * 32 + q;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = fmaf(f, p[e * 32], v[e]);
@@ -163,7 +167,7 @@ struct Split {  // what both kernels start with
         regions = (float*)(smem + IMG);
         region = smem + IMG + (size_t)wave * REGION;
         ml = (float*)(smem + IMG + (size_t)nw * REGION);
-        codes = (int*)(ml + nw * 96);
+        codes = (int*)(ml + nw * 128);
         bias = (float*)(codes + ((N + 31) >> 5) * 32);
         b = blockIdx.x / H, h = blockIdx.x - b * H;
         const int hk = h / (H / a.HK);
@@ -302,7 +306,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(DH <= 64 ? 
 
 // LDS of a workgroup of nw waves, and how many waves fit (one always does)
 size_t split_lds(int dh, int size, int nw, int N, int slice) {
-    return split_image(dh, size) + (size_t)nw * (split_region(dh, size) + 384) + ((size_t)(N + 31) / 32 * 32 + slice) * 4;
+    return split_image(dh, size) + (size_t)nw * (split_region(dh, size) + 512) + ((size_t)(N + 31) / 32 * 32 + slice) * 4;
 }
 int split_waves(int dh, int size, int N, int slice, int most) {
     const int nt = ceil_div(N, 32);

@@ -166,6 +166,11 @@ struct RelLevel {
         const bool up = excess(mx, c) > 0.f;
         const float p = mx * c;
         const bool f = fabsf(p) > kRelFar;
+        if (!far && !__any(up && f)) {
+            const float m1 = fmaxf(m, p), factor = __builtin_amdgcn_exp2f(m - m1);
+            m = m1;
+            return factor;
+        }
         const float M1 = up ? f ? mx : 0.f : M, m1 = up ? f ? 0.f : p : m;
         const float factor = __builtin_amdgcn_exp2f(fmaf(M - M1, c, m - m1));
         M = M1;
