@@ -79,8 +79,8 @@ constexpr int chunk_bytes() { return 2 * CR * LdsImage<DH>::ROW + (MODE == MODE_
 template <int DH, int MODE>
 __device__ __forceinline__ void chunk_products(const RelBwdArgs& a, const unsigned char* buf, int img, int ro, const TrRead<DH>& tr,
                                                const RelLane<MODE == MODE_DQ>& rl, const bf16x8 (&f1)[DH / 16], const bf16x8 (&f2)[DH / 16], bool far,
-                                               const float* Mr, float oL, float oD, f32x16 (&acc1)[(DH + 31) / 32], f32x16 (&acc2)[(DH + 31) / 32], float& dsum, int row0, int nb,
-                                               int hi) {
+                                               const float* Mr, float oL, float oD, f32x16 (&acc1)[(DH + 31) / 32],
+                                               f32x16 (&acc2)[(DH + 31) / 32], float& dsum, int row0, int nb, int hi) {
     using I = LdsImage<DH>;
     constexpr int KS = DH / 16, DB = (DH + 31) / 32, IMG = CR * I::ROW, BUF = chunk_bytes<DH, MODE>();
     f32x16 s, dp;
