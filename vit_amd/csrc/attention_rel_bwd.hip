@@ -342,8 +342,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves_p
 
 // ---- sums of dS over samples, folded by offset. Grid: (query blocks * key blocks, H, splits). A wave has 32 queries and KT tiles of
 // 32 keys; K and V of the block's keys come by LDS-DMA one sample ahead (two buffers), the wave's own Q and dO rows one sample ahead
-// in registers, so a sample costs one barrier and its loads have a sample's products to land. 256 x 197 tokens, 12 heads of 64: 116 us,
-// 4 x 1025, 16 heads of 80: 99 us (of a workgroup's 80 000 cycles there 17 000 go by before the first product, 10 000 in the fold). Folded a
+// in registers, so a sample costs one barrier and its loads have a sample's products to land. 256 x 197 tokens, 12 heads of 64: 115 us,
+// 4 x 1025, 16 heads of 80: 98 us (of a workgroup's 80 000 cycles there 17 000 go by before the first product, 10 000 in the fold). Folded a
 // strip of 32 keys at a time by the whole workgroup it took 1.1 and 1.25 times as long.
 template <int DH, int KT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2))) void attn_rel_bias_grad_kernel(const RelBwdArgs a) {

@@ -7,7 +7,7 @@
 // Two barriers an item, all loads a phase ahead: the next item's K, V images and every wave's own Q, dO, O rows (registers) come under B,
 // whose images are Q and dO; those come under A, whose images are K and V (an L2 hit: the rows went to registers one phase before).
 //
-// 256 x 197 tokens, 12 heads: 246 us for 620 MB and 7 products of 32 x 32 x 64 a pair of tiles. Bound by each wave's chain of matrix and
+// 256 x 197 tokens, 12 heads: 245 us for 620 MB and 7 products of 32 x 32 x 64 a pair of tiles. Bound by each wave's chain of matrix and
 // vector instructions (two waves a SIMD with 252 registers each; those two kinds overlap by about 30 %). As two chunked launches: 152 +
 // 207 us. Fragments fetched a tile ahead or two tiles a step spilled and took longer; waves started at an offset gained 2 %.
 #include "lds_image.h"

@@ -8,8 +8,8 @@
 // workgroup meets once or twice, behind a barrier pair of its own.
 //
 // Bound by the waves' own chains (about 140 vector instructions of 4 cycles and 16 exponentials beside 8 matrix instructions a tile, of
-// which a quarter overlap). 256 x 197 tokens, 12 heads: 89 us (310 MB: 3.5 TB/s; attention without a bias 77 us); 32 x 577, 16 heads: 102 us
-// (0.43 PFLOP/s; without 77 us). Whole-sequence images staged at once took 142 and 173 us; the idle eighth wave's place passed round the SIMDs gained
+// which a quarter overlap). 256 x 197 tokens, 12 heads: 90 us (310 MB: 3.4 TB/s; attention without a bias 77 us); 32 x 577, 16 heads: 100 us
+// (0.44 PFLOP/s; without 77 us). Whole-sequence images staged at once took 142 and 173 us; the idle eighth wave's place passed round the SIMDs gained
 // nothing.
 #include "rel_bias.h"
 #include <math.h>

@@ -12,8 +12,8 @@
 // weights of those 8 values are loaded once per token / once per wave. Row sums are DPP adds inside 2..16 lanes, the
 // rotation's partner values come from a lane of the same head.
 //
-// 256 x 197 tokens, 12 + 12 heads of 64, bf16, RMS: forward 88 us for 464 MB (5.3 TB/s, what a large copy reaches), backward 119 us for
-// 620 MB (5.2 TB/s); 9 x 331 tokens, 12 + 4 heads of 96, LayerNorm, positions: 9.2 us, of which 4.4 are its bytes: the loads' chain of one
+// 256 x 197 tokens, 12 + 12 heads of 64, bf16, RMS: forward 87 us for 464 MB (5.3 TB/s, what a large copy reaches), backward 117 us for
+// 620 MB (5.3 TB/s); 9 x 331 tokens, 12 + 4 heads of 96, LayerNorm, positions: 9.2 us, of which 4.4 are its bytes: the loads' chain of one
 // token a wave (heads before weights: 15.2 us the other way round); fp32 backward of 3 x 1025 tokens, 16 + 16 heads of 80: 30 us for 126 MB
 // that come from HBM, 26 us where an earlier call left them in the caches. The parameters' sums are fp32 (in a fixed order).
 #include "vit_common.h"
